@@ -340,6 +340,80 @@ int32_t splat_selftest_bounded_wait(int32_t* status_word, int64_t limit_cycles, 
  * SPLAT/r_sddmm.py:24-37, SPLAT/r_spmm.py:24-38). */
 int32_t splat_debug_check_indices(int32_t* status_word);
 
+/* ---------------------------------------------------------------------------------------------
+ * Serving: a paged cache of keys and values, and rotary positions.  No counterpart in the reference.
+ *
+ * The cache holds K and V in pages of `page` rows; a row is one token's d elements of one K/V head, contiguous.  Pages, heads and
+ * rows lie at any strides (in elements).  Token j of request b is row j mod page of page block_table[b][j / page]; an entry outside
+ * [0, pages) is a page that is not there: its keys are not attended to, and nothing is written to it.
+ * ------------------------------------------------------------------------------------------- */
+#define SPLAT_PAGED_MAX_REQUESTS 16384
+#define SPLAT_ROTARY_MAX_AXES 4
+
+/* Block tables, slots and positions of a step.  Request b has ctx_lens[b] tokens in the cache and brings q_lens[b] (negative
+ * lengths count as 0).  Pages that it needs in addition are taken from `ring`, in the order of the requests: the free ones are
+ * ring[i mod ring_size] for span[0] <= i < span[1].  Written: the new entries of block_table (requests rows of table_stride, width
+ * entries), kv_lens = ctx + q, q_start (requests + 1, exclusive sums of q_lens), taken = {span[0] behind the step, span[1], pages
+ * that were missing}, and for each of `tokens` rows its slot (page * page + row, or -1), position and request; rows behind
+ * the last request get -1, 0 and -1.  A page that is missing (ring empty, table too narrow) leaves -1 in the table and the slots.
+ * Outputs may not overlap inputs; the inputs but block_table stay as they are. */
+int32_t splat_paged_tables(const int32_t* ctx_lens, const int32_t* q_lens, int32_t* block_table, int64_t table_stride,
+                           const int32_t* ring, int64_t ring_size, const int64_t* span, int64_t page, int64_t requests,
+                           int64_t width, int64_t tokens, int32_t* kv_lens, int32_t* q_start, int64_t* slots,
+                           int32_t* positions, int32_t* token_request, int64_t* taken, void* stream);
+
+/* Rows in, rows out: element c of head h, batch b, token l at src + b * src_b + h * src_h + l * src_l + c.  turned: by the
+ * positions (otherwise copied).  paged: dst is a cache and dst_b, dst_h, dst_l are its page, head and row strides. */
+typedef struct {
+    const void* src;
+    void* dst;
+    int64_t heads;
+    int64_t src_b, src_h, src_l;
+    int64_t dst_b, dst_h, dst_l;
+    int32_t turned, paged;
+} splat_rows;
+
+/* Rotary positions on 1 to 3 arrays of rows.  Pair i of a row (elements i and i + half, or 2 i and 2 i + 1 with `interleaved`) turns
+ * by positions[axis(i)] * inv_freq[i], the other way with `inverse`; sections (host memory, axes entries that add up to half) says
+ * how many pairs in turn go by each axis.  positions: int32, or int64 with positions_64, at axis * pos_axis + b * pos_b + l * pos_l.
+ * Elements behind the first 2 * half are copied.  dst may be src.  slots: (batch * length), the cache rows of `paged` arrays; a
+ * slot outside [0, pages * page) is left out, and two tokens may not have the same one. */
+int32_t splat_rotary(const splat_rows* rows, int32_t n_rows, const void* positions, int32_t positions_64, int64_t pos_axis,
+                     int64_t pos_b, int64_t pos_l, const float* inv_freq, int64_t half, const int64_t* sections,
+                     int32_t axes, int32_t interleaved, int32_t inverse, int64_t batch, int64_t length, int64_t d,
+                     int32_t dtype, const int64_t* slots, int64_t page, int64_t pages, void* stream);
+
+/* Attention of new tokens over the paged cache.  Request b's queries are rows q_start[b] .. q_start[b + 1] - 1 of q, its last tokens:
+ * query row t stands at position i = kv_lens[b] - q_start[b + 1] + t and attends to the keys j = i - k * stride >= 0, k < taps
+ * (taps = 0: all of them).  Score: x = scale q.k, capped to softcap tanh(x / softcap) if softcap > 0, less slopes[head] (i - j) if
+ * slopes is not null.  Query head h reads K/V head h / (heads / kv_heads).  o: softmax of the scores times V, 0 for a query without a
+ * key; lse: (tokens, heads) float32 or null, the natural log-sum-exp of the scores, -inf for a query without a key.  Rows of q in
+ * front of the first request and behind the last, and those of a request whose rows do not lie within [0, tokens), are left as they are. */
+typedef struct {
+    const void *q, *k_cache, *v_cache;
+    void* o;
+    float* lse;
+    int64_t q_row, q_head, o_row, o_head;                    /* strides in elements; last dimension contiguous */
+    int64_t k_page, k_head, k_row, v_page, v_head, v_row;
+    const int32_t* block_table;
+    int64_t table_stride, table_width;
+    const int32_t* kv_lens;
+    const int32_t* q_start;                                  /* requests + 1 entries, or null: one token each */
+    const float* slopes;                                     /* heads entries, or null */
+    int64_t tokens, requests, pages, page, heads, kv_heads, d;
+    int64_t taps, stride;
+    int64_t max_q_len;                                       /* no request brings more (longer ones are still right) */
+    float scale, softcap;
+    int32_t dtype;
+    int32_t* status_word;                                    /* see splat_attention_fused; or null */
+    void* workspace;                                         /* splat_paged_attention_workspace bytes, 16-byte aligned */
+    int64_t workspace_bytes;
+} splat_paged_args;
+
+/* Bytes of device memory that the call works in; they may hold anything before and after it. */
+int64_t splat_paged_attention_workspace(const splat_paged_args* args);
+int32_t splat_paged_attention(const splat_paged_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,188 @@
+"""CPU: what the paged cache's and the rotary positions' launchers refuse, and their oracle against itself."""
+import random
+
+import pytest
+import torch
+
+import r_paged
+import r_rotary
+from oracle import paged_oracle as po
+
+
+def i32(*shape):
+    return torch.zeros(shape, dtype=torch.int32)
+
+
+def i64(*shape):
+    return torch.zeros(shape, dtype=torch.int64)
+
+
+def refused(call, kw, change, words, error=ValueError):
+    kw = {**kw, **change}
+    with pytest.raises(error, match=words):
+        call(**kw)
+
+
+def tables_args():
+    return dict(ctx_lens=i32(3), q_lens=i32(3), block_table=i32(3, 5), free_pages=i32(9), free_span=i64(2), page_size=16,
+                kv_lens=i32(3), q_start=i32(4), slots=i64(7), positions=i32(7), requests=i32(7), free_span_out=i64(3))
+
+
+@pytest.mark.parametrize("change, words, error", [
+    (dict(), "CUDA devices only", ValueError),
+    (dict(q_lens=i32(2)), "q_lens and ctx_lens", ValueError),
+    (dict(ctx_lens=i64(3)), "ctx_lens must be int32", TypeError),
+    (dict(slots=i32(7)), "slots must be int64", TypeError),
+    (dict(q_start=i32(3)), "q_start", ValueError),
+    (dict(block_table=i32(2, 5)), "a row for each request", ValueError),
+    (dict(block_table=i32(1, 5).expand(3, 5)), "must not overlap", ValueError),
+    (dict(block_table=i32(5, 3).t()), "last dimension", ValueError),
+    (dict(page_size=0), "page_size must be at least 1", ValueError),
+    (dict(page_size=1.5), "integer", TypeError),
+    (dict(free_pages=i32(0)), "must not be empty", ValueError),
+    (dict(free_span=i64(3)), "2 entries", ValueError),
+    (dict(free_span_out=i64(2)), "3 entries", ValueError),
+    (dict(positions=i32(6)), "differ in length", ValueError),
+    (dict(ctx_lens=i32(6)[::2]), "contiguous", ValueError),
+    (dict(ctx_lens=[1, 2, 3]), "must be a tensor", TypeError),
+    (dict(ctx_lens=i32(20000), q_lens=i32(20000), kv_lens=i32(20000), q_start=i32(20001), block_table=i32(20000, 1)),
+     "at most", ValueError),
+])
+def test_tables_refusals(change, words, error):
+    refused(r_paged.rpaged_tables_launcher, tables_args(), change, words, error)
+
+
+def rotary_args():
+    return dict(q=torch.zeros(2, 4, 6, 16), k=torch.zeros(2, 2, 6, 16), positions=i32(3, 2, 6), inv_freq=torch.zeros(8),
+                sections=(4, 2, 2))
+
+
+@pytest.mark.parametrize("change, words, error", [
+    (dict(), "CUDA devices only", ValueError),
+    (dict(k=torch.zeros(2, 2, 5, 16)), "must agree", ValueError),
+    (dict(k=torch.zeros(2, 2, 6, 16).half()), "dtype", TypeError),
+    (dict(q=torch.zeros(2, 4, 6, 16).double()), "unsupported dtype", TypeError),
+    (dict(q=torch.zeros(4, 6, 16)), "4-dimensional", ValueError),
+    (dict(q=torch.zeros(2, 4, 16, 6).transpose(2, 3)), "last dimension", ValueError),
+    (dict(positions=i32(3, 2, 5)), "differ in length", ValueError),
+    (dict(positions=i32(3, 1, 6)), "differ in batch", ValueError),
+    (dict(positions=torch.zeros(3, 2, 6)), "int32 or int64", TypeError),
+    (dict(positions=i32(5, 2, 6), sections=(2, 2, 2, 1, 1)), "1 to 4 axes", ValueError),
+    (dict(sections=(4, 4)), "an entry for each axis", ValueError),
+    (dict(sections=(4, 2, 1)), "add up", ValueError),
+    (dict(sections=(10, -1, -1)), "at least 0", ValueError),
+    (dict(sections=None), "must be given", ValueError),
+    (dict(inv_freq=torch.zeros(9), sections=(5, 2, 2)), "only 16 elements", ValueError),
+    (dict(inv_freq=torch.zeros(8).double()), "float32", TypeError),
+])
+def test_rotary_refusals(change, words, error):
+    refused(r_rotary.rrotary_launcher, rotary_args(), change, words, error)
+    refused(r_rotary.rrotary, rotary_args(), change, words, error)
+
+
+def test_rotary_refuses_gradients_of_the_frequencies_and_expanded_outputs():
+    kw = rotary_args()
+    kw["inv_freq"].requires_grad_(True)
+    refused(r_rotary.rrotary, kw, {}, "no.* for the frequencies")
+    refused(r_rotary.rrotary_launcher, rotary_args(), dict(q_out=torch.zeros(1, 4, 6, 16).expand(2, 4, 6, 16)), "expanded")
+    refused(r_rotary.rrotary_launcher, rotary_args(), dict(q_out=torch.zeros(2, 4, 6, 8)), "shape")
+
+
+def append_args():
+    return dict(q=torch.zeros(5, 4, 16), k=torch.zeros(5, 2, 16), v=torch.zeros(5, 2, 16), k_cache=torch.zeros(3, 2, 8, 16),
+                v_cache=torch.zeros(3, 2, 8, 16), slots=i64(5), q_out=torch.zeros(5, 4, 16), positions=i32(2, 5),
+                inv_freq=torch.zeros(8), sections=(5, 3))
+
+
+@pytest.mark.parametrize("change, words, error", [
+    (dict(), "CUDA devices only", ValueError),
+    (dict(slots=i64(4)), "differ in length", ValueError),
+    (dict(slots=i32(5)), "int64", TypeError),
+    (dict(v=torch.zeros(5, 3, 16)), "same shape", ValueError),
+    (dict(k_cache=torch.zeros(3, 1, 8, 16), v_cache=torch.zeros(3, 1, 8, 16)), "differ in heads", ValueError),
+    (dict(k_cache=torch.zeros(3, 2, 8, 8), v_cache=torch.zeros(3, 2, 8, 8)), "differ in length", ValueError),
+    (dict(k_cache=torch.zeros(3, 2, 8, 16).half()), "dtype", TypeError),
+    (dict(k_cache=torch.zeros(1, 2, 8, 16).expand(3, 2, 8, 16)), "expanded", ValueError),
+    (dict(k_cache=torch.zeros(3, 2, 16, 8).transpose(2, 3)), "last dimension", ValueError),
+    (dict(q_out=None), "q_out must be a tensor", TypeError),
+    (dict(q=None), "q_out without q", ValueError),
+    (dict(q_out=torch.zeros(5, 4, 8)), "shape of q", ValueError),
+    (dict(positions=None), "inv_freq without positions", ValueError),
+    (dict(inv_freq=None), "positions without inv_freq", ValueError),
+    (dict(positions=i32(2, 4)), "differ in length", ValueError),
+    (dict(positions=i32(2, 1, 5)), "axes, tokens", ValueError),
+])
+def test_append_refusals(change, words, error):
+    refused(r_paged.rpaged_append_launcher, append_args(), change, words, error)
+
+
+def attention_args():
+    return dict(q=torch.zeros(5, 4, 16), k_cache=torch.zeros(3, 2, 8, 16), v_cache=torch.zeros(3, 2, 8, 16),
+                block_table=i32(2, 4), kv_lens=i32(2), output=torch.zeros(5, 4, 16), q_start=i32(3))
+
+
+@pytest.mark.parametrize("change, words, error", [
+    (dict(), "CUDA devices only", ValueError),
+    (dict(q_start=None), "one token for each request", ValueError),
+    (dict(q_start=i32(2)), "one entry more", ValueError),
+    (dict(q_start=i64(3)), "int32", TypeError),
+    (dict(q=torch.zeros(5, 3, 16), output=torch.zeros(5, 3, 16)), "multiple", ValueError),
+    (dict(output=torch.zeros(5, 4, 8)), "shape of q", ValueError),
+    (dict(output=torch.zeros(5, 4, 32)[..., ::2]), "output must be contiguous", ValueError),
+    (dict(output=torch.zeros(5, 4, 16).half()), "dtype", TypeError),
+    (dict(v_cache=torch.zeros(3, 2, 4, 16)), "same shape", ValueError),
+    (dict(block_table=i32(1, 4)), "a row for each request", ValueError),
+    (dict(kv_lens=i64(2)), "int32", TypeError),
+    (dict(taps=-1), "taps must be at least 0", ValueError),
+    (dict(stride=0), "stride must be at least 1", ValueError),
+    (dict(softcap=-1.0), "softcap must not be negative", ValueError),
+    (dict(scale=float("nan")), "scale must be finite", ValueError),
+    (dict(scale=1e300), "scale must be finite", ValueError),
+    (dict(slopes=torch.zeros(2)), "an entry for each head", ValueError),
+    (dict(slopes=torch.zeros(4).half()), "float32", TypeError),
+    (dict(lse=torch.zeros(4, 5)), "lse must have shape", ValueError),
+    (dict(max_q_len=-1), "max_q_len must be at least 0", ValueError),
+    (dict(q=torch.zeros(5, 4, 257), output=torch.zeros(5, 4, 257), k_cache=torch.zeros(3, 2, 8, 257),
+          v_cache=torch.zeros(3, 2, 8, 257)), "1 to 256", ValueError),
+    (dict(k_cache=torch.zeros(1, 2, 1, 16).expand(1, 2, 1 << 29, 16), v_cache=torch.zeros(1, 2, 1, 16).expand(1, 2, 1 << 29, 16)),
+     "beyond what the kernels count", ValueError),
+])
+def test_attention_refusals(change, words, error):
+    refused(r_paged.rpaged_attention_launcher, attention_args(), change, words, error)
+
+
+def test_module_refuses_the_cpu():
+    with pytest.raises(ValueError, match="CUDA devices only"):
+        r_paged.PagedAttention(4, 16, 4, 2, 64, 2, 8, 64, "cpu", torch.float16)
+
+
+def test_oracle_tables_hand_out_each_page_once():
+    rng = random.Random(5)
+    for _ in range(50):
+        page, B = rng.choice([1, 3, 16]), rng.randrange(1, 6)
+        ctx = [rng.randrange(40) for _ in range(B)]
+        new = [rng.randrange(-2, 30) for _ in range(B)]
+        width = 80
+        held = [-(-c // page) for c in ctx]
+        free = list(range(1000, 1000 + rng.randrange(1, 120)))
+        table, at = [], 0
+        for h in held:
+            table.append([at + i if i < h else -7 for i in range(width)])
+            at += h
+        got = po.tables(ctx, new, table, free, [11, 11 + len(free)], page, 200)
+        used = [p for row, c, n in zip(got["table"], ctx, new) for p in row[:-(-(c + max(n, 0)) // page)] if p >= 0]
+        assert len(used) == len(set(used))
+        live = [s for s in got["slots"] if s >= 0]
+        assert len(live) == len(set(live))
+        assert got["taken"][0] - 11 + got["taken"][2] == sum(-(-(c + max(n, 0)) // page) - h for c, n, h in zip(ctx, new, held))
+
+
+def test_oracle_rotary_turns_back():
+    g = torch.Generator().manual_seed(1)
+    x = torch.randn(2, 3, 5, 12, generator=g, dtype=torch.float64)
+    pos = torch.randint(0, 50000, (2, 2, 5), generator=g)
+    freq = torch.rand(5, generator=g)
+    for interleaved in (False, True):
+        y = po.rotary(x, pos, freq, (2, 3), interleaved)
+        assert torch.allclose(po.rotary(y, pos, freq, (2, 3), interleaved, inverse=True), x)
+        assert torch.equal(y[..., 10:], x[..., 10:])

@@ -74,11 +74,17 @@ SIGNATURES = {
                                     _i64, _i64, _f32, _i32, _i32, _vp, _vp, _vp, _vp, _vp],
     "splat_attention_noalloc": [_vp, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _i64,
                                 _i64, _i64, _i64, _f32, _i32, _vp],
+    "splat_paged_tables": [_vp, _vp, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _i64] + [_vp] * 7,
+    "splat_rotary": [_vp, _i32, _vp, _i32, _i64, _i64, _i64, _vp, _i64, _vp, _i32, _i32, _i32, _i64, _i64, _i64, _i32,
+                     _vp, _i64, _i64, _vp],
+    "splat_paged_attention_workspace": [_vp],
+    "splat_paged_attention": [_vp, _vp],
 }
 for _name, _args in SIGNATURES.items():
     _fn = getattr(_lib, _name)
     _fn.argtypes = _args
     _fn.restype = _i32
+_lib.splat_paged_attention_workspace.restype = _i64
 _lib.splat_status_string.argtypes = [_i32]
 _lib.splat_status_string.restype = ctypes.c_char_p
 
@@ -654,3 +660,21 @@ _host.bind(*(ctypes.cast(getattr(_lib, name), _vp).value for name in (
     "splat_attention_fused_table", "splat_sddmm_band_table", "splat_spmm_band_table", "splat_sddmm_tile_status",
     "splat_spmm_tile_status",
     "splat_softmax", "splat_acsr_from_mask_u8", "splat_transpose_16", "splat_sddmm", "splat_spmm")), _warn_cuda_core_16bit)
+
+
+# ----------------------------------------------------------------------------------------------
+# paged cache and rotary positions: checked and launched by native code (csrc/paged_binding.cpp)
+# ----------------------------------------------------------------------------------------------
+def _prepare_paged(index: int) -> None:
+    """Before a launch whose kernels have bounded waits: the device's status word, unless a graph is captured (the
+    kernels without such waits run then), and what an earlier kernel reported through it."""
+    dev = torch.device("cuda", index)
+    _raise_if_gave_up(dev)
+    _native_from_now_on(dev)
+
+
+_host.bind_paged(*(ctypes.cast(getattr(_lib, name), _vp).value for name in (
+    "splat_paged_tables", "splat_rotary", "splat_paged_attention_workspace", "splat_paged_attention",
+    "splat_status_string")), _prepare_paged)
+paged_tables, paged_append, paged_attention = _host.paged_tables, _host.paged_append, _host.paged_attention
+rotary = _host.rotary

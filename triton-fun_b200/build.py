@@ -3,7 +3,7 @@
     python triton-fun_b200/build.py [--force] [--verbose]
 
 The library is a plain C-ABI shared object (see include/splat_b200.h); it does not link torch.
-splat_host is the Python extension module behind the launchers (csrc/host_binding.cpp): it reads torch's
+splat_host is the Python extension module behind the launchers (csrc/host_binding.cpp, csrc/paged_binding.cpp): it reads torch's
 tensors and calls the library, and is compiled against the installed torch.
 """
 from __future__ import annotations
@@ -18,7 +18,8 @@ REPO_ROOT = os.path.dirname(PKG_DIR)
 CSRC = os.path.join(PKG_DIR, "csrc")
 INCLUDE = os.path.join(REPO_ROOT, "include")
 LIB_PATH = os.path.join(PKG_DIR, "libsplat_b200.so")
-HOST_SRC = os.path.join(CSRC, "host_binding.cpp")
+HOST_SRCS = [os.path.join(CSRC, f) for f in ("host_binding.cpp", "paged_binding.cpp")]
+HOST_HDRS = [os.path.join(CSRC, "paged_binding.h"), os.path.join(INCLUDE, "splat_b200.h")]
 HOST_PATH = os.path.join(PKG_DIR, "SPLAT", "splat_host.so")
 HOST_BUILT_FOR = HOST_PATH + ".built-for"      # the torch and Python that it was compiled against
 
@@ -51,7 +52,7 @@ def build_host(force: bool = False) -> str:
     import torch
     built_for = f"torch {torch.__version__}, Python {sys.version}"
     if not force and os.path.exists(HOST_PATH) and os.path.exists(HOST_BUILT_FOR) and \
-            all(os.path.getmtime(f) <= os.path.getmtime(HOST_PATH) for f in (HOST_SRC, __file__)):
+            all(os.path.getmtime(f) <= os.path.getmtime(HOST_PATH) for f in (*HOST_SRCS, *HOST_HDRS, __file__)):
         with open(HOST_BUILT_FOR) as f:
             if f.read() == built_for:
                 return HOST_PATH
@@ -62,7 +63,7 @@ def build_host(force: bool = False) -> str:
            "-I" + os.path.join(root, "include"),
            "-I" + os.path.join(root, "include", "torch", "csrc", "api", "include"),
            "-I" + os.path.join(cuda, "include"), "-I" + sysconfig.get_paths()["include"],
-           HOST_SRC, "-o", HOST_PATH, "-L" + os.path.join(root, "lib"),
+           "-I" + INCLUDE, *HOST_SRCS, "-o", HOST_PATH, "-L" + os.path.join(root, "lib"),
            "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python"]
     print(" ".join(cmd), file=sys.stderr)
     subprocess.run(cmd, check=True)

@@ -27,6 +27,8 @@
 #include <exception>
 #include <mutex>
 
+#include "paged_binding.h"
+
 namespace {
 
 constexpr int kPathAuto = 0, kPathGeneric = 1, kPathBand = 2;
@@ -576,6 +578,11 @@ PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "splat_host", nullptr, -1, meth
 
 }  // namespace
 
+namespace splat_host {
+int32_t* status_word(int device) { return device >= 0 && device < kMaxDevices ? g_status[device].word : nullptr; }
+bool status_ready(int device) { return status_word(device) != nullptr && *g_status[device].mirror == 0; }
+}  // namespace splat_host
+
 PyMODINIT_FUNC PyInit_splat_host() {
     k_lin = PyUnicode_InternFromString("sTod_linear_transformations");
     k_tr = PyUnicode_InternFromString("sTod_translations");
@@ -586,5 +593,10 @@ PyMODINIT_FUNC PyInit_splat_host() {
     k_plan = PyUnicode_InternFromString("plan");
     k_lse = PyUnicode_InternFromString("lse");
     k_cached_plan = PyUnicode_InternFromString("_splat_plan");
-    return PyModule_Create(&module_def);
+    PyObject* module = PyModule_Create(&module_def);
+    if (module != nullptr && PyModule_AddFunctions(module, splat_host::paged_methods()) != 0) {
+        Py_DECREF(module);
+        return nullptr;
+    }
+    return module;
 }

@@ -1,0 +1,397 @@
+// Attention of new tokens over a paged cache: the entry points, the kernel for any operands, and the joining of divided tiles.
+//
+// For query position i of head h, over the keys j = i - k stride >= 0 with k < taps:
+//     x_j = c tanh(scale q.k_j / c) or scale q.k_j;   s_j = x_j - slope_h (i - j);   o = sum_j e^(s_j - m) v_j / sum_j e^(s_j - m)
+// with m the running maximum; scores, sums and outputs are held in fp32, in powers of two.  How the work is divided: paged_schedule.cuh.
+#include <initializer_list>
+
+#include "paged_schedule.cuh"
+
+namespace splat {
+namespace paged {
+
+__device__ __forceinline__ float score_of(const Problem& p, float dot) {
+    return p.softcap > 0.f ? p.softcap * tanhf(dot * p.cap_inv) : dot * p.scale_log2;
+}
+
+// -------------------------------------------------------------------------------------------------
+// Any type, d up to 256, any strides and alignment: FP32 FMA.  It is what fp32 runs on, and 16-bit operands that the tensor-core
+// kernels cannot fetch.
+//
+// A tile is 8 rows.  kLanes lanes (16 for d <= 64, else the warp) hold a key: each has kCols of its columns and of the 8 rows' q and o.  The
+// 8 dot products are added up over the lanes by halving: 4 + 2 + 1 exchanges leave every lane with one row's sum over some lanes, one
+// or two more complete it (8 to 9 shuffles for 8 sums; one by one they would be 32 to 40).  Four keys are in flight per stream; a
+// block's 4 warps are 4 or 8 streams that share a tile's keys and are joined at its end.
+// -------------------------------------------------------------------------------------------------
+constexpr int kRowsAny = 8, kKeysAny = 32, kThreadsAny = 128, kBatchAny = 4;
+
+template <int kLanes> __device__ __forceinline__ float reduce_rows(const float (&v)[kRowsAny], int lane) {
+    float w[4], x[2], y;
+    const bool a = lane & (kLanes / 2), b = lane & (kLanes / 4), c = lane & (kLanes / 8);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = (a ? v[i + 4] : v[i]) + __shfl_xor_sync(0xffffffffu, a ? v[i] : v[i + 4], kLanes / 2);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) x[i] = (b ? w[i + 2] : w[i]) + __shfl_xor_sync(0xffffffffu, b ? w[i] : w[i + 2], kLanes / 4);
+    y = (c ? x[1] : x[0]) + __shfl_xor_sync(0xffffffffu, c ? x[0] : x[1], kLanes / 8);
+#pragma unroll
+    for (int o = kLanes / 16; o > 0; o >>= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
+    return y;
+}
+// the lane of a group that holds row r's sum
+template <int kLanes> __device__ __forceinline__ int lane_of_row(int r) {
+    return (r & 4 ? kLanes / 2 : 0) + (r & 2 ? kLanes / 4 : 0) + (r & 1 ? kLanes / 8 : 0);
+}
+
+template <typename T, int kCols>
+__device__ __forceinline__ void load_cols(const T* row, int col0, int d, bool wide, float (&x)[kCols]) {
+    if (wide) {                        // (rows and d in whole pieces of kCols elements)
+        if (col0 < d) {
+            constexpr int kPiece = kCols * (int)sizeof(T) < 16 ? kCols * (int)sizeof(T) : 16;
+            constexpr int kEach = kPiece / (int)sizeof(T);
+#pragma unroll
+            for (int i = 0; i < kCols; i += kEach) {
+                T e[kEach];
+                if constexpr (kPiece == 16) *reinterpret_cast<uint4*>(e) = *reinterpret_cast<const uint4*>(row + col0 + i);
+                else *reinterpret_cast<uint2*>(e) = *reinterpret_cast<const uint2*>(row + col0 + i);
+#pragma unroll
+                for (int j = 0; j < kEach; ++j) x[i + j] = DT<T>::to_f(e[j]);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < kCols; ++i) x[i] = 0.f;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < kCols; ++i) x[i] = col0 + i < d ? DT<T>::to_f(row[col0 + i]) : 0.f;
+    }
+}
+
+template <typename T, int kLanes, int kCols>
+__global__ void __launch_bounds__(kThreadsAny) paged_rows_kernel(const Problem p, const bool wide) {
+    constexpr int kStreams = kThreadsAny / kLanes, kD = kLanes * kCols;
+    using Part = Walk<kRowsAny, kKeysAny, kThreadsAny>;
+    __shared__ union Shared {
+        WalkShared<kThreadsAny> walk;
+        struct { float m[kStreams][kRowsAny], l[kStreams][kRowsAny], o[kStreams][kRowsAny][kD]; } join;
+    } sh;
+    const int lane = threadIdx.x & 31, in_group = lane & (kLanes - 1), stream = threadIdx.x / kLanes;
+    const int col0 = in_group * kCols;
+    depend_wait();
+    depend_release();
+    Part w;
+    const bool any = w.start(p, sh.walk);
+    if (threadIdx.x == 0) p.begins[blockIdx.x] = any && w.at != w.tile_begin ? w.tile_begin : -1;
+    if (!any) return;
+    const int g = (int)p.group.d, s = (int)p.stride.d;
+    do {
+        const TileRows t = TileRows::of(p, w);
+        const int32_t* table = p.table + w.b * p.table_stride;
+        // this lane's row, and all rows' q
+        const int own = ((in_group & (kLanes / 2)) ? 4 : 0) + ((in_group & (kLanes / 4)) ? 2 : 0) + ((in_group & (kLanes / 8)) ? 1 : 0);
+        auto token_of = [&](int r) {                       // index of the row's token in its class, or -1
+            const int m = p.group.div(w.tile * kRowsAny + r);
+            return m < t.count ? m : -1;
+        };
+        auto head_of = [&](int r, int m) { return w.head * g + w.tile * kRowsAny + r - m * g; };
+        float q[kRowsAny][kCols], o[kRowsAny][kCols];
+#pragma unroll
+        for (int r = 0; r < kRowsAny; ++r) {
+            const int m = token_of(r);
+#pragma unroll
+            for (int i = 0; i < kCols; ++i) q[r][i] = o[r][i] = 0.f;
+            if (m >= 0)
+                load_cols<T, kCols>(static_cast<const T*>(p.q) + (w.r.first + w.cls + (int64_t)m * s) * p.q_row + (int64_t)head_of(r, m) * p.q_head,
+                                    col0, p.d, wide, q[r]);
+        }
+        const int own_m = token_of(own);
+        const int own_u = own_m >= 0 ? t.u0 + own_m : INT32_MIN / 2;                   // sees keys (own_u - taps, own_u]
+        const float slope = own_m >= 0 && p.slopes != nullptr ? p.slopes[head_of(own, own_m)] * kLog2e * (float)s : 0.f;
+        const int m_first = token_of(0), m_last = min(p.group.div(w.tile * kRowsAny + kRowsAny - 1), t.count - 1);
+        const int lo = max(m_first < 0 ? 0 : t.u0 + m_first - p.taps + 1, w.first_step() * kKeysAny);
+        const int hi = m_first < 0 ? 0 : min(t.u0 + m_last + 1, w.last_step() * kKeysAny);
+        float top = -INFINITY, sum = 0.f;                   // of the lane's row, over the stream's keys
+        const T* kb = static_cast<const T*>(p.k) + w.head * p.k_head;
+        const T* vb = static_cast<const T*>(p.v) + w.head * p.v_head;
+        for (int n0 = max(lo, 0); n0 < hi; n0 += kStreams * kBatchAny) {               // (the same for all threads: shuffles inside)
+            const int n = n0 + stream * kBatchAny;
+            float x[kBatchAny];
+            int64_t at[kBatchAny];
+            bool edge = false;
+            {
+                float k[kBatchAny][kCols];
+#pragma unroll
+                for (int i = 0; i < kBatchAny; ++i) {
+                    at[i] = n + i < hi ? cache_row(p, table, t.residue + (int64_t)(n + i) * s, p.k_page, p.k_row) : -1;
+#pragma unroll
+                    for (int c = 0; c < kCols; ++c) k[i][c] = 0.f;
+                    if (at[i] >= 0) load_cols<T, kCols>(kb + at[i], col0, p.d, wide, k[i]);
+                }
+#pragma unroll
+                for (int i = 0; i < kBatchAny; ++i) {
+                    float dot[kRowsAny];
+#pragma unroll
+                    for (int r = 0; r < kRowsAny; ++r) {
+                        dot[r] = 0.f;
+#pragma unroll
+                        for (int c = 0; c < kCols; ++c) dot[r] = fmaf(q[r][c], k[i][c], dot[r]);
+                    }
+                    x[i] = reduce_rows<kLanes>(dot, in_group);
+                }
+            }
+            float most = top;
+#pragma unroll
+            for (int i = 0; i < kBatchAny; ++i) {
+                const bool seen = at[i] >= 0 && n + i <= own_u && n + i > own_u - p.taps;
+                x[i] = seen ? score_of(p, x[i]) - slope * (float)(own_u - n - i) : -INFINITY;
+                edge = edge || !seen;
+                most = fmaxf(most, x[i]);
+            }
+            edge = __any_sync(0xffffffffu, edge);
+            const float base = most == -INFINITY ? 0.f : most, corr = exp2f(top - base);
+            const bool moved = __any_sync(0xffffffffu, most > top);
+            top = most;
+#pragma unroll
+            for (int i = 0; i < kBatchAny; ++i) x[i] = x[i] == -INFINITY ? 0.f : exp2f(x[i] - base);
+            if (moved) {
+                sum *= corr;
+#pragma unroll
+                for (int r = 0; r < kRowsAny; ++r) {
+                    const float f = __shfl_sync(0xffffffffu, corr, (lane & ~(kLanes - 1)) | lane_of_row<kLanes>(r));
+#pragma unroll
+                    for (int c = 0; c < kCols; ++c) o[r][c] *= f;
+                }
+            }
+            float v[kBatchAny][kCols];
+#pragma unroll
+            for (int i = 0; i < kBatchAny; ++i) {
+#pragma unroll
+                for (int c = 0; c < kCols; ++c) v[i][c] = 0.f;
+                if (at[i] >= 0)
+                    load_cols<T, kCols>(vb + cache_row(p, table, t.residue + (int64_t)(n + i) * s, p.v_page, p.v_row), col0, p.d, wide, v[i]);
+            }
+#pragma unroll
+            for (int i = 0; i < kBatchAny; ++i) {
+                sum += x[i];
+#pragma unroll
+                for (int r = 0; r < kRowsAny; ++r) {
+                    const float f = __shfl_sync(0xffffffffu, x[i], (lane & ~(kLanes - 1)) | lane_of_row<kLanes>(r));
+                    // a key that a row does not see may hold anything: 0 times infinity would be NaN
+                    if (!edge || f != 0.f) {
+#pragma unroll
+                        for (int c = 0; c < kCols; ++c) o[r][c] = fmaf(f, v[i][c], o[r][c]);
+                    }
+                }
+            }
+        }
+        // the streams' parts, joined
+        __syncthreads();
+        if ((in_group & (kLanes / 8 - 1)) == 0) {
+            sh.join.m[stream][own] = top;
+            sh.join.l[stream][own] = sum;
+        }
+#pragma unroll
+        for (int r = 0; r < kRowsAny; ++r)
+#pragma unroll
+            for (int c = 0; c < kCols; ++c) sh.join.o[stream][r][col0 + c] = o[r][c];
+        __syncthreads();
+        const bool whole = w.whole();
+        const int64_t part = w.part();
+        for (int i = threadIdx.x; i < kRowsAny * kD; i += kThreadsAny) {
+            const int r = i / kD, c = i - r * kD, m = token_of(r);
+            float most = -INFINITY, all = 0.f, y = 0.f;
+            for (int j = 0; j < kStreams; ++j) most = fmaxf(most, sh.join.m[j][r]);
+            const float base = most == -INFINITY ? 0.f : most;
+            for (int j = 0; j < kStreams; ++j) {
+                const float f = exp2f(sh.join.m[j][r] - base);
+                all = fmaf(f, sh.join.l[j][r], all);
+                y = fmaf(f, sh.join.o[j][r][c], y);
+            }
+            const int token = m >= 0 ? w.r.first + w.cls + m * s : -1, head = m >= 0 ? head_of(r, m) : 0;
+            if (!whole) {
+                if (c == 0) p.part_rows[part * kRowsAny + r] = make_float4(most, all, __int_as_float(token), __int_as_float(head));
+                p.part_o[(part * kRowsAny + r) * kD + c] = y;
+            } else if (token >= 0) {
+                if (c < p.d)
+                    static_cast<T*>(p.o)[token * p.o_row + head * p.o_head + c] = DT<T>::from_f(all != 0.f ? y / all : 0.f);
+                if (c == 0 && p.lse != nullptr)
+                    p.lse[(int64_t)token * p.kv_heads * g + head] = all == 0.f ? -INFINITY : (most + log2f(all)) * kLn2;
+            }
+        }
+        __syncthreads();
+    } while (w.next(p));
+}
+
+// -------------------------------------------------------------------------------------------------
+// Parts of divided tiles -> results.  Block (c, y): the tile that CTA c begins in the middle of, if no CTA before it does too; a warp per
+// row.  It runs behind the kernel that wrote them, as a launch that is already waiting when that ends.
+// -------------------------------------------------------------------------------------------------
+constexpr int kThreadsJoin = 256;
+
+template <typename T, int kD>
+__global__ void __launch_bounds__(kThreadsJoin) paged_join_kernel(const Problem p, const int ctas, const int rows) {
+    constexpr int kEach = (kD + 127) / 128;                // pieces of 4 columns of a lane
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = blockIdx.x + 1;
+    depend_wait();
+    depend_release();
+    const int64_t id = p.begins[c];
+    if (id < 0 || p.begins[c - 1] == id) return;
+    int n = 1;                                             // parts
+    for (int j = c; j < ctas; j += 32) {
+        const unsigned same = __ballot_sync(0xffffffffu, j + lane < ctas && p.begins[min(j + lane, ctas - 1)] == id);
+        n += __popc(same);
+        if (same != 0xffffffffu) break;
+    }
+    auto part = [&](int i) { return (int64_t)(i == 0 ? 2 * (c - 1) + 1 : 2 * (c - 1 + i)); };
+    for (int r = blockIdx.y * (kThreadsJoin / 32) + warp; r < rows; r += gridDim.y * (kThreadsJoin / 32)) {
+        const float4 first = p.part_rows[part(0) * rows + r];
+        const int token = __float_as_int(first.z), head = __float_as_int(first.w);
+        if (token < 0) continue;
+        float most = -INFINITY;
+        for (int i = lane; i < n; i += 32) most = fmaxf(most, p.part_rows[part(i) * rows + r].x);
+        most = warp_max(most);
+        const float base = most == -INFINITY ? 0.f : most;
+        float all = 0.f, o[kEach][4];
+#pragma unroll
+        for (int e = 0; e < kEach; ++e)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) o[e][k] = 0.f;
+        for (int i0 = 0; i0 < n; i0 += 32) {
+            float f = 0.f;
+            if (i0 + lane < n) {
+                const float4 x = p.part_rows[part(i0 + lane) * rows + r];
+                f = exp2f(x.x - base);
+                all += f * x.y;
+            }
+            const int here = min(32, n - i0);
+#pragma unroll 8
+            for (int i = 0; i < here; ++i) {
+                const float fi = __shfl_sync(0xffffffffu, f, i);
+#pragma unroll
+                for (int e = 0; e < kEach; ++e) {
+                    const int col = e * 128 + lane * 4;
+                    if (col < kD) {
+                        const float4 x = *reinterpret_cast<const float4*>(p.part_o + (part(i0 + i) * rows + r) * kD + col);
+                        o[e][0] = fmaf(fi, x.x, o[e][0]);
+                        o[e][1] = fmaf(fi, x.y, o[e][1]);
+                        o[e][2] = fmaf(fi, x.z, o[e][2]);
+                        o[e][3] = fmaf(fi, x.w, o[e][3]);
+                    }
+                }
+            }
+        }
+        all = warp_sum(all);
+        T* out = static_cast<T*>(p.o) + token * p.o_row + head * p.o_head;
+#pragma unroll
+        for (int e = 0; e < kEach; ++e)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int col = e * 128 + lane * 4 + k;
+                if (col < p.d) out[col] = DT<T>::from_f(all != 0.f ? o[e][k] / all : 0.f);
+            }
+        if (lane == 0 && p.lse != nullptr)
+            p.lse[(int64_t)token * p.kv_heads * (int)p.group.d + head] = all == 0.f ? -INFINITY : (most + log2f(all)) * kLn2;
+    }
+}
+
+template <typename T>
+static int32_t join_as(const Problem& p, int ctas, int rows, int d_pad, cudaStream_t st) {
+    const dim3 grid((unsigned)(ctas - 1), (unsigned)((rows + kThreadsJoin / 32 - 1) / (kThreadsJoin / 32)));
+    auto kern = d_pad == 64 ? paged_join_kernel<T, 64> : d_pad == 128 ? paged_join_kernel<T, 128> : paged_join_kernel<T, 256>;
+    return launch_kernel(kern, grid, dim3(kThreadsJoin), 0, st, p, ctas, rows);
+}
+int32_t join_parts(const Problem& p, int ctas, int rows, int d_pad, int32_t dtype, cudaStream_t st) {
+    if (ctas < 2) return SPLAT_OK;
+    if (dtype == SPLAT_F32) return join_as<float>(p, ctas, rows, d_pad, st);
+    if (dtype == SPLAT_F16) return join_as<__half>(p, ctas, rows, d_pad, st);
+    return join_as<__nv_bfloat16>(p, ctas, rows, d_pad, st);
+}
+
+// -------------------------------------------------------------------------------------------------
+// Host side
+// -------------------------------------------------------------------------------------------------
+static int sm_count() {
+    int dev = 0, n = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) {
+        (void)cudaGetLastError();
+        return 0;
+    }
+    return n;
+}
+
+constexpr int kPerSmAny = 3;
+static int d_pad_any(int64_t d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
+
+template <typename T>
+static int32_t launch_any(const splat_paged_args& a, Problem p, int ctas, cudaStream_t st) {
+    p.rows_from = 0;
+    p.rows_to = INT32_MAX;
+    constexpr int kCols = 4;
+    const int64_t piece = a.d <= 128 ? kCols : 2 * kCols, bytes = piece * sizeof(T) < 16 ? piece * sizeof(T) : 16, e = bytes / sizeof(T);
+    auto fits = [&](const void* x, std::initializer_list<int64_t> strides) {
+        bool ok = reinterpret_cast<uintptr_t>(x) % bytes == 0;
+        for (int64_t s : strides) ok = ok && s % e == 0;
+        return ok;
+    };
+    const bool wide = a.d % piece == 0 && fits(a.q, {a.q_row, a.q_head}) && fits(a.k_cache, {a.k_page, a.k_head, a.k_row}) &&
+                      fits(a.v_cache, {a.v_page, a.v_head, a.v_row});
+    Layout(ctas, kRowsAny, d_pad_any(a.d)).place(p, a.workspace);
+    auto kern = a.d <= 64 ? paged_rows_kernel<T, 16, kCols> : a.d <= 128 ? paged_rows_kernel<T, 32, kCols> : paged_rows_kernel<T, 32, 2 * kCols>;
+    const int32_t rc = launch_kernel(kern, dim3((unsigned)ctas), dim3(kThreadsAny), 0, st, p, wide);
+    return rc != SPLAT_OK ? rc : join_parts(p, ctas, kRowsAny, d_pad_any(a.d), a.dtype, st);
+}
+
+static int32_t check_args(const splat_paged_args& a) {
+    if (a.dtype != SPLAT_F32 && a.dtype != SPLAT_F16 && a.dtype != SPLAT_BF16) return SPLAT_ERR_UNSUPPORTED_DTYPE;
+    if (a.tokens < 0 || a.requests < 0 || a.pages < 0 || a.page < 1 || a.heads < 1 || a.kv_heads < 1 || a.d < 1 || a.taps < 0 || a.stride < 1 ||
+        a.table_width < 0 || a.table_stride < a.table_width || a.heads % a.kv_heads != 0 || !(a.softcap >= 0.f))
+        return SPLAT_ERR_BAD_ARG;
+    if (a.requests > SPLAT_PAGED_MAX_REQUESTS || a.d > 256 || a.pages > INT32_MAX || a.page > kMaxLen || a.table_width > kMaxLen ||
+        a.table_width * a.page > kMaxLen || a.heads > 65535 || a.tokens >= kMaxLen / a.heads)
+        return SPLAT_ERR_UNSUPPORTED_SHAPE;
+    return SPLAT_OK;
+}
+
+}  // namespace paged
+}  // namespace splat
+
+extern "C" int64_t splat_paged_attention_workspace(const splat_paged_args* a) {
+    using namespace splat::paged;
+    if (!a || check_args(*a) != SPLAT_OK) return 0;
+    return Layout(sm_count() * kPerSmAny, kRowsAny, d_pad_any(a->d)).bytes;
+}
+
+extern "C" int32_t splat_paged_attention(const splat_paged_args* args, void* stream) {
+    using namespace splat;
+    using namespace splat::paged;
+    if (!args) return SPLAT_ERR_BAD_ARG;
+    const splat_paged_args& a = *args;
+    if (const int32_t rc = check_args(a); rc != SPLAT_OK) return rc;
+    if (a.tokens == 0 || a.requests == 0) return SPLAT_OK;
+    if (!a.q || !a.o || !a.kv_lens || (a.table_width > 0 && !a.block_table) || (a.pages > 0 && a.table_width > 0 && (!a.k_cache || !a.v_cache)))
+        return SPLAT_ERR_BAD_ARG;
+    const int sms = sm_count();
+    if (sms < 1) return SPLAT_ERR_NO_DEVICE;
+    if (!a.workspace || !aligned16(a.workspace) || a.workspace_bytes < splat_paged_attention_workspace(args)) return SPLAT_ERR_SCRATCH_TOO_SMALL;
+    Problem p = {};
+    p.q = a.q; p.k = a.k_cache; p.v = a.v_cache; p.o = a.o; p.lse = a.lse;
+    p.q_row = a.q_row; p.q_head = a.q_head; p.o_row = a.o_row; p.o_head = a.o_head;
+    p.k_page = a.k_page; p.k_head = a.k_head; p.k_row = a.k_row;
+    p.v_page = a.v_page; p.v_head = a.v_head; p.v_row = a.v_row;
+    p.table = a.block_table; p.table_stride = a.table_stride;
+    p.kv_lens = a.kv_lens; p.q_start = a.q_start; p.slopes = a.slopes;
+    p.tokens = (int)a.tokens; p.requests = (int)a.requests; p.pages = (int)a.pages; p.page = (int)a.page;
+    p.kv_heads = (int)a.kv_heads; p.d = (int)a.d;
+    p.table_rows = (int)(a.table_width * a.page);
+    p.taps = a.taps == 0 || a.taps > kAllTaps ? kAllTaps : (int)a.taps;
+    p.group = FastDiv((uint32_t)(a.heads / a.kv_heads));
+    p.stride = FastDiv((uint32_t)(a.stride < kMaxLen ? a.stride : kMaxLen));
+    p.page_div = FastDiv((uint32_t)a.page);
+    p.scale_log2 = a.scale * kLog2e;
+    p.softcap = a.softcap * kLog2e;
+    p.cap_inv = a.softcap > 0.f ? a.scale / a.softcap : 0.f;
+    cudaStream_t st = (cudaStream_t)stream;
+    const int ctas = sms * kPerSmAny;
+    if (a.dtype == SPLAT_F32) return launch_any<float>(a, p, ctas, st);
+    if (a.dtype == SPLAT_F16) return launch_any<__half>(a, p, ctas, st);
+    return launch_any<__nv_bfloat16>(a, p, ctas, st);
+}

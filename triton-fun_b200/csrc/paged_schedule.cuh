@@ -1,0 +1,251 @@
+// How the attention over a paged cache is divided over CTAs (paged_attention.cu, paged_chunk.cu).
+//
+// Query position i attends to the keys i, i - stride, i - 2 stride, ...  So a request's tokens fall into residue classes modulo the
+// stride, and a class is a problem of stride 1: token m of class c (the tokens c, c + stride, ... of the request's new ones) has
+// index u0 + m among the keys residue, residue + stride, ... and attends to the keys u0 + m - taps + 1 .. u0 + m of them.
+// A tile is R rows of one class and one K/V head; a row is a (token, query head of the group) pair, the group's heads of a token behind one
+// another, so that every key is fetched once for all of them.  A tile's keys are walked over in steps of kKeys.
+//
+// The lengths are on the device only.  Every CTA reads them all, counts the steps of all tiles and takes an equal, contiguous share of
+// them, whatever tiles it begins and ends in: a decoding batch of ragged lengths, a few long requests and one long prompt all keep
+// the whole GPU busy, and nothing has to be planned on the host or in another launch.  Tiles that several CTAs work on are joined by
+// paged_join_kernel from (maximum, sum, unnormalised output) of each part; a CTA has two of those at most, of its first and of its last
+// tile.  The parts of a tile are added up in the order of its keys: results do not depend on timing, though they do, in the last
+// bits, on what else is in the batch.
+//
+// Steps are counted for a class of a request's longest kind, so that all of its classes and heads have the same tiles; where the count
+// is one too high a CTA has a step without keys.
+#pragma once
+
+#include "common.cuh"
+
+namespace splat {
+namespace paged {
+
+struct FastDiv {               // n / d for 0 <= n < 2^31
+    uint32_t mul, shift, d;
+    FastDiv() = default;
+    explicit FastDiv(uint32_t d_) : d(d_) {
+        shift = 0;
+        while ((1ull << shift) < d) ++shift;
+        mul = (uint32_t)(((1ull << 32) * ((1ull << shift) - d)) / d + 1);
+    }
+    __device__ __forceinline__ int div(int n) const { return (int)((__umulhi(mul, (uint32_t)n) + (uint32_t)n) >> shift); }
+    __device__ __forceinline__ int div_floor(int n) const { return n >= 0 ? div(n) : -1 - div(-1 - n); }
+};
+
+constexpr int kMaxLen = 1 << 30;       // of a request, in tokens
+constexpr int kAllTaps = 1 << 30;
+
+struct Problem {
+    const void *q, *k, *v;
+    void* o;
+    float* lse;
+    int64_t q_row, q_head, o_row, o_head;
+    int64_t k_page, k_head, k_row, v_page, v_head, v_row;
+    const int32_t* table;
+    int64_t table_stride;
+    const int32_t* kv_lens;
+    const int32_t* q_start;
+    const float* slopes;
+    int tokens, requests, pages, page, kv_heads, d;
+    int table_rows;                    // tokens that the table has room for
+    int taps;
+    FastDiv group, stride, page_div;   // query heads per K/V head
+    int rows_from, rows_to;            // requests with so many rows in a class are this kernel's
+    float scale_log2, softcap, cap_inv;    // x = qk * scale_log2, or softcap_log2 * tanh(qk * cap_inv)
+    // workspace
+    int64_t* begins;                   // per CTA: first step of the tile that it begins in the middle of, or -1
+    float4* part_rows;                 // [2 per CTA][R] maximum, sum, token, query head
+    float* part_o;                     // [2 per CTA][R][D]
+    int32_t* status;                   // of kernels with bounded waits
+    int32_t* mirror;
+};
+
+struct Request {
+    int first, n;                      // rows of q
+    int pos;                           // position of the first
+    int classes, longest;              // classes; tokens of the longest
+    int tiles;                         // of a class
+    int u0;                            // index of the first token of class 0
+};
+
+template <int R>
+__device__ __forceinline__ Request request_of(const Problem& p, int b) {
+    Request r;
+    int t0 = b, t1 = b + 1;
+    if (p.q_start != nullptr) { t0 = __ldg(p.q_start + b); t1 = __ldg(p.q_start + b + 1); }
+    const int kv = min(max(__ldg(p.kv_lens + b), 0), kMaxLen);
+    r.first = t0;
+    r.n = t0 >= 0 && t1 <= p.tokens && t1 > t0 ? t1 - t0 : 0;
+    r.pos = kv - r.n;
+    const int s = (int)p.stride.d, g = (int)p.group.d;
+    r.classes = min(s, r.n);
+    r.longest = p.stride.div(r.n + s - 1);
+    const int64_t rows = (int64_t)r.longest * g;
+    if (rows < p.rows_from || rows > p.rows_to) r.n = r.classes = r.longest = 0;
+    r.tiles = (int)(((int64_t)r.longest * g + R - 1) / R);
+    r.u0 = p.stride.div_floor(r.pos);
+    return r;
+}
+
+// Steps [x, y) of kKeys keys that a tile of class c counts for.
+template <int R, int kKeys>
+__device__ __forceinline__ int2 steps_of(const Problem& p, const Request& r, int tile) {
+    const int m_lo = p.group.div(tile * R), m_hi = min(p.group.div(tile * R + R - 1), r.longest - 1);
+    const int lo = max(0, r.u0 + m_lo - p.taps + 1), hi = r.u0 + m_hi + (p.stride.d > 1 ? 2 : 1);
+    const int x = lo / kKeys;
+    return make_int2(x, max(x + 1, (hi + kKeys - 1) / kKeys));
+}
+template <int R, int kKeys>
+__device__ __forceinline__ int64_t steps_of_class(const Problem& p, const Request& r) {
+    int64_t sum = 0;
+    for (int t = 0; t < r.tiles; ++t) {
+        const int2 s = steps_of<R, kKeys>(p, r, t);
+        sum += s.y - s.x;
+    }
+    return sum;
+}
+__device__ __forceinline__ int64_t divide(int64_t a, int64_t b) {
+    return ((a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
+}
+
+template <int kThreads> struct WalkShared {
+    int64_t before[kThreads + 1];      // steps in front of a thread's requests
+    int64_t warp_sums[kThreads / 32];
+};
+
+// A CTA's walk over its share.  All threads of the block, the same in each.
+template <int R, int kKeys, int kThreads>
+struct Walk {
+    int64_t at, end;                   // steps, of all
+    int64_t tile_begin;                // of the tile that `at` is in
+    int b, head, cls, tile;
+    Request r;
+    int2 steps;                        // of the tile
+    int64_t class_steps;
+
+    // Scans the lengths; false if there is nothing to do for this CTA.
+    __device__ bool start(const Problem& p, WalkShared<kThreads>& sh) {
+        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+        const int each = (p.requests + kThreads - 1) / kThreads;
+        int64_t mine = 0;
+        for (int i = 0; i < each; ++i) {
+            const int q = threadIdx.x * each + i;
+            if (q >= p.requests) break;
+            const Request x = request_of<R>(p, q);
+            mine += steps_of_class<R, kKeys>(p, x) * x.classes * p.kv_heads;
+        }
+        int64_t x = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o) x += y;
+        }
+        if (lane == 31) sh.warp_sums[warp] = x;
+        __syncthreads();
+        for (int w = 0; w < warp; ++w) x += sh.warp_sums[w];
+        sh.before[threadIdx.x + 1] = x;
+        if (threadIdx.x == 0) sh.before[0] = 0;
+        __syncthreads();
+        const int64_t all = sh.before[kThreads], share = divide(all + gridDim.x - 1, gridDim.x);
+        at = min((int64_t)blockIdx.x * share, all);
+        end = min(at + share, all);
+        if (at >= end) return false;
+        int lo = 0, hi = kThreads;     // the last thread whose requests begin at or before `at`
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (sh.before[mid] <= at) lo = mid; else hi = mid;
+        }
+        int64_t sum = sh.before[lo];
+        for (b = lo * each;; ++b) {    // (ends: the steps behind `at` are some request's)
+            r = request_of<R>(p, b);
+            class_steps = steps_of_class<R, kKeys>(p, r);
+            const int64_t w = class_steps * r.classes * p.kv_heads;
+            if (at < sum + w) break;
+            sum += w;
+        }
+        int64_t rest = at - sum;
+        const int64_t per_head = class_steps * r.classes;
+        head = (int)divide(rest, per_head);
+        rest -= head * per_head;
+        cls = (int)divide(rest, class_steps);
+        rest -= cls * class_steps;
+        for (tile = 0;; ++tile) {
+            steps = steps_of<R, kKeys>(p, r, tile);
+            if (rest < steps.y - steps.x) break;
+            rest -= steps.y - steps.x;
+        }
+        tile_begin = at - rest;
+        return true;
+    }
+    __device__ __forceinline__ int first_step() const { return steps.x + (int)(at - tile_begin); }
+    __device__ __forceinline__ int last_step() const { return (int)min((int64_t)steps.y, steps.x + (end - tile_begin)); }    // (one behind)
+    __device__ __forceinline__ bool whole() const { return at == tile_begin && end - tile_begin >= steps.y - steps.x; }
+    __device__ __forceinline__ int part() const { return 2 * blockIdx.x + (at == tile_begin ? 1 : 0); }
+    // To the next tile; false at the end of the share.
+    __device__ bool next(const Problem& p) {
+        at = tile_begin + (steps.y - steps.x);
+        if (at >= end) return false;
+        tile_begin = at;
+        if (++tile == r.tiles) {
+            tile = 0;
+            if (++cls == r.classes) {
+                cls = 0;
+                if (++head == p.kv_heads) {
+                    head = 0;
+                    do r = request_of<R>(p, ++b); while (r.n == 0);      // (ends: `at` is before the share's end)
+                }
+            }
+        }
+        steps = steps_of<R, kKeys>(p, r, tile);
+        return true;
+    }
+};
+
+// What a tile's rows and keys are.
+struct TileRows {
+    int count;                         // tokens of the class
+    int u0;                            // index of its first among the class's keys
+    int residue;                       // key n of the class is token residue + n * stride
+    template <int R, int K, int N> __device__ __forceinline__ static TileRows of(const Problem& p, const Walk<R, K, N>& w) {
+        TileRows t;
+        const int s = (int)p.stride.d, pos = w.r.pos + w.cls;
+        t.count = p.stride.div(w.r.n - w.cls + s - 1);
+        t.u0 = p.stride.div_floor(pos);
+        t.residue = pos - t.u0 * s;
+        return t;
+    }
+};
+
+// Row of K or V of token j of request b: offset into the cache (without the head), or -1 if it is not there.
+__device__ __forceinline__ int64_t cache_row(const Problem& p, const int32_t* table, int64_t j, int64_t page_stride, int64_t row_stride) {
+    if (j >= p.table_rows) return -1;
+    const int i = p.page_div.div((int)j);
+    const int page = __ldg(table + i);
+    if (page < 0 || page >= p.pages) return -1;
+    return page * page_stride + ((int)j - i * (int)p.page_div.d) * row_stride;
+}
+
+// What a kernel of this kind needs of workspace.
+struct Layout {
+    int64_t begins, rows, o, bytes;
+    Layout(int ctas, int tile_rows, int d) {
+        begins = 0;
+        rows = (ctas * 8 + 15) / 16 * 16;
+        o = rows + (int64_t)2 * ctas * tile_rows * 16;
+        bytes = o + (int64_t)2 * ctas * tile_rows * d * 4;
+    }
+    void place(Problem& p, void* workspace) const {
+        char* w = static_cast<char*>(workspace);
+        p.begins = reinterpret_cast<int64_t*>(w + begins);
+        p.part_rows = reinterpret_cast<float4*>(w + rows);
+        p.part_o = reinterpret_cast<float*>(w + o);
+    }
+};
+
+// Joins the parts of divided tiles, written by `ctas` CTAs with tiles of tile_rows rows and d_pad columns.  Defined in paged_attention.cu.
+int32_t join_parts(const Problem& p, int ctas, int tile_rows, int d_pad, int32_t dtype, cudaStream_t st);
+
+}  // namespace paged
+}  // namespace splat
