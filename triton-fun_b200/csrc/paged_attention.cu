@@ -5,7 +5,7 @@
 // with m the running maximum; scores, sums and outputs are held in fp32, in powers of two.  How the work is divided: paged_schedule.cuh.
 #include <initializer_list>
 
-#include "paged_schedule.cuh"
+#include "paged_rows.cuh"
 
 namespace splat {
 namespace paged {
@@ -23,7 +23,7 @@ __device__ __forceinline__ float score_of(const Problem& p, float dot) {
 // or two more complete it (8 to 9 shuffles for 8 sums; one by one they would be 32 to 40).  Four keys are in flight per stream; a
 // block's 4 warps are 4 or 8 streams that share a tile's keys and are joined at its end.
 // -------------------------------------------------------------------------------------------------
-constexpr int kRowsAny = 8, kKeysAny = 32, kThreadsAny = 128, kBatchAny = 4;
+constexpr int kRowsAny = 8, kKeysAny = 32, kThreadsAny = 128, kBatchAny = 4, kFixedAny = 3;
 
 template <int kLanes> __device__ __forceinline__ float reduce_rows(const float (&v)[kRowsAny], int lane) {
     float w[4], x[2], y;
@@ -69,7 +69,7 @@ __device__ __forceinline__ void load_cols(const T* row, int col0, int d, bool wi
 template <typename T, int kLanes, int kCols>
 __global__ void __launch_bounds__(kThreadsAny) paged_rows_kernel(const Problem p, const bool wide) {
     constexpr int kStreams = kThreadsAny / kLanes, kD = kLanes * kCols;
-    using Part = Walk<kRowsAny, kKeysAny, kThreadsAny>;
+    using Part = Walk<kRowsAny, kKeysAny, kThreadsAny, kFixedAny>;
     __shared__ union Shared {
         WalkShared<kThreadsAny> walk;
         struct { float m[kStreams][kRowsAny], l[kStreams][kRowsAny], o[kStreams][kRowsAny][kD]; } join;
@@ -80,7 +80,7 @@ __global__ void __launch_bounds__(kThreadsAny) paged_rows_kernel(const Problem p
     depend_release();
     Part w;
     const bool any = w.start(p, sh.walk);
-    if (threadIdx.x == 0) p.begins[blockIdx.x] = any && w.at != w.tile_begin ? w.tile_begin : -1;
+    if (threadIdx.x == 0) p.begins[blockIdx.x] = any && !w.begins() ? w.tile_begin : -1;
     if (!any) return;
     const int g = (int)p.group.d, s = (int)p.stride.d;
     do {
@@ -323,8 +323,6 @@ static int d_pad_any(int64_t d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
 
 template <typename T>
 static int32_t launch_any(const splat_paged_args& a, Problem p, int ctas, cudaStream_t st) {
-    p.rows_from = 0;
-    p.rows_to = INT32_MAX;
     constexpr int kCols = 4;
     const int64_t piece = a.d <= 128 ? kCols : 2 * kCols, bytes = piece * sizeof(T) < 16 ? piece * sizeof(T) : 16, e = bytes / sizeof(T);
     auto fits = [&](const void* x, std::initializer_list<int64_t> strides) {
@@ -351,13 +349,55 @@ static int32_t check_args(const splat_paged_args& a) {
     return SPLAT_OK;
 }
 
+// What the tensor-core kernels can fetch: 16-byte pieces of K and V.
+static bool tensor_cores(const splat_paged_args& a) {
+    auto pieces = [](int64_t x, int64_t y, int64_t z) { return x % 8 == 0 && y % 8 == 0 && z % 8 == 0; };
+    return a.dtype != SPLAT_F32 && a.pages > 0 && a.d % 8 == 0 && a.d <= 128 && aligned16(a.k_cache) && aligned16(a.v_cache) && aligned16(a.o) &&
+           pieces(a.k_page, a.k_head, a.k_row) && pieces(a.v_page, a.v_head, a.v_row) && pieces(a.o_row, a.o_head, 0);
+}
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                  const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+int box_rows(const splat_paged_args& a, int most) {
+    if (a.stride > a.page || a.page % a.stride != 0) return 0;
+    const int64_t rows = a.page / a.stride, power = rows & -rows;
+    const int box = (int)(power < most ? power : most);
+    return box >= 8 ? box : 0;
+}
+bool cache_map(CUtensorMap* map, const splat_paged_args& a, const void* base, int64_t page, int64_t head, int64_t row, int rows) {
+    static const EncodeTiledFn fn = [] {
+        void* f = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) f = nullptr;
+        return reinterpret_cast<EncodeTiledFn>(f);
+    }();
+    if (fn == nullptr) return false;
+    const int64_t class_rows = a.page / a.stride;
+    const cuuint64_t dims[5] = {(cuuint64_t)a.d, (cuuint64_t)a.stride, (cuuint64_t)class_rows, (cuuint64_t)a.kv_heads, (cuuint64_t)a.pages};
+    cuuint64_t strides[4] = {(cuuint64_t)(row * 2), (cuuint64_t)(a.stride * row * 2), (cuuint64_t)(head * 2), (cuuint64_t)(page * 2)};
+    for (int i = 0; i < 4; ++i) {
+        if (dims[i + 1] == 1) strides[i] = (cuuint64_t)(a.d * 2);      // (never stepped over)
+        if (strides[i] == 0) return false;                             // an expanded cache
+    }
+    const cuuint32_t box[5] = {64, 1, (cuuint32_t)rows, 1, 1}, each[5] = {1, 1, 1, 1, 1};
+    return fn(map, a.dtype == SPLAT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5, const_cast<void*>(base), dims, strides,
+              box, each, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// paged_decode.cu
+int decode_ctas(int sms);
+int32_t attend_decode(const splat_paged_args& a, Problem p, int sms, void* workspace, cudaStream_t st);
+
 }  // namespace paged
 }  // namespace splat
 
 extern "C" int64_t splat_paged_attention_workspace(const splat_paged_args* a) {
     using namespace splat::paged;
     if (!a || check_args(*a) != SPLAT_OK) return 0;
-    return Layout(sm_count() * kPerSmAny, kRowsAny, d_pad_any(a->d)).bytes;
+    const int sms = sm_count();
+    if (tensor_cores(*a)) return Layout(decode_ctas(sms), 16, d_pad_any(a->d)).bytes;
+    return Layout(sms * kPerSmAny, kRowsAny, d_pad_any(a->d)).bytes;
 }
 
 extern "C" int32_t splat_paged_attention(const splat_paged_args* args, void* stream) {
@@ -389,8 +429,13 @@ extern "C" int32_t splat_paged_attention(const splat_paged_args* args, void* str
     p.scale_log2 = a.scale * kLog2e;
     p.softcap = a.softcap * kLog2e;
     p.cap_inv = a.softcap > 0.f ? a.scale / a.softcap : 0.f;
+    p.status = a.status_word;
+    p.mirror = a.status_word != nullptr ? status_mirror(a.status_word) : nullptr;
     cudaStream_t st = (cudaStream_t)stream;
     const int ctas = sms * kPerSmAny;
+    p.rows_from = 0;
+    p.rows_to = INT32_MAX;
+    if (tensor_cores(a)) return attend_decode(a, p, sms, a.workspace, st);
     if (a.dtype == SPLAT_F32) return launch_any<float>(a, p, ctas, st);
     if (a.dtype == SPLAT_F16) return launch_any<__half>(a, p, ctas, st);
     return launch_any<__nv_bfloat16>(a, p, ctas, st);

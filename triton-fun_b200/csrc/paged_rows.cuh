@@ -1,0 +1,138 @@
+// Rows of a tile in the kernels of the paged attention on tensor cores: where they stand, how a result leaves, and a row's result from
+// its own keys alone.
+#pragma once
+
+#include <cuda.h>
+
+#include "paged_schedule.cuh"
+#include "softmax_math.cuh"
+#include "tc_ptx.cuh"
+
+namespace splat {
+namespace band { bool allow_dynamic_smem(const void* kernel, int bytes); }      // attention_band.cu
+
+namespace paged {
+
+// Rows of a tiled copy from the cache for chunks of up to `most` (a power of two) keys: so many that a page's rows of one residue class are
+// whole boxes, at least 8 (a box's rows are exchanged in groups of 8); 0 if there are none.
+int box_rows(const splat_paged_args& a, int most);
+// The cache as (columns, residues, rows of a class in a page, heads, pages), boxes of 64 columns and `rows` rows.  False if it cannot be
+// described so.  Both in paged_attention.cu.
+bool cache_map(CUtensorMap* map, const splat_paged_args& a, const void* base, int64_t page, int64_t head, int64_t row, int rows);
+
+__device__ __forceinline__ void load_box(uint32_t smem_dst, const CUtensorMap* map, uint64_t* bar, int column, int residue, int row, int head, int page) {
+    asm volatile(
+        "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], [%2];" ::"r"(smem_dst),
+        "l"(map), "r"(tc::smem_u32(bar)), "r"(column), "r"(residue), "r"(row), "r"(head), "r"(page)
+        : "memory");
+}
+
+// Row r of a tile: token m of its class, query head of the group.
+template <int R> struct RowPlace {
+    int first, last;                   // tokens of the tile (first may be the class's count: no rows)
+    int base, g, head0, count, stride;
+    int64_t row0;
+    FastDiv group;
+    template <int K, int N, int F>
+    __device__ __forceinline__ RowPlace(const Problem& p, const Walk<R, K, N, F>& w, const TileRows& t) {
+        base = w.tile * R;
+        g = (int)p.group.d;
+        group = p.group;
+        head0 = w.head * g;
+        count = t.count;
+        stride = (int)p.stride.d;
+        row0 = w.r.first + w.cls;
+        first = min(group.div(base), count);
+        last = min(group.div(base + R - 1), count - 1);
+    }
+    __device__ __forceinline__ int token_of(int r) const {             // or -1
+        const int m = group.div(base + r);
+        return m < count ? m : -1;
+    }
+    __device__ __forceinline__ int head_of(int r, int m) const { return head0 + base + r - m * g; }
+    __device__ __forceinline__ int64_t row_of(int m) const { return row0 + (int64_t)m * stride; }
+};
+
+// c tanh(x / c) in the log2 domain, with tanh y = 1 - 2 / (e^2y + 1): off by some 2^-22 of c, as the scores are by their sums.
+__device__ __forceinline__ float capped(const Problem& p, float dot) {
+    const float e = sm::ex2(dot * p.cap_inv * (2.f * kLog2e));
+    return p.softcap - __fdividef(2.f * p.softcap, e + 1.f);
+}
+
+// Four columns of a finished row, or of a part of one (index `slot` of the parts).
+template <typename T>
+__device__ __forceinline__ void put_row(const Problem& p, bool whole, int64_t slot, int d_pad, int token, int head, int col, float top, float sum, float4 y) {
+    if (!whole) {
+        if (col == 0) p.part_rows[slot] = make_float4(top, sum, __int_as_float(token), __int_as_float(head));
+        *reinterpret_cast<float4*>(p.part_o + slot * d_pad + col) = y;
+        return;
+    }
+    if (token < 0) return;
+    if (col < p.d) {                   // (d is a multiple of 8, and the output contiguous)
+        const float inv = sum != 0.f ? 1.f / sum : 0.f;
+        uint2 out = make_uint2(sm::pack2<T>(y.x * inv, y.y * inv), sm::pack2<T>(y.z * inv, y.w * inv));
+        *reinterpret_cast<uint2*>(static_cast<T*>(p.o) + token * p.o_row + head * p.o_head + col) = out;
+    }
+    if (col == 0 && p.lse != nullptr)
+        p.lse[(int64_t)token * p.kv_heads * (int)p.group.d + head] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
+}
+
+// Row r of the tile over its own keys in [lo, hi), by one warp.  A tile multiplies keys that a row does not see with probability 0, and 0
+// times infinity is NaN; such rows are rare, are noticed at the end, and come here.
+template <typename T, int D, int R>
+__device__ __noinline__ void row_again(const Problem& p, int kv_head, const int32_t* table, const TileRows t, const RowPlace<R> rows, int r, int lo,
+                                       int hi, bool whole, int64_t slot) {
+    const int lane = threadIdx.x & 31, s = (int)p.stride.d;
+    const int m = rows.token_of(r), head = rows.head_of(r, m), u = t.u0 + m;
+    lo = max(lo, u - p.taps + 1);
+    hi = min(hi, u + 1);
+    const float slope = p.slopes != nullptr ? p.slopes[head] * kLog2e * (float)s : 0.f;
+    const T* q = static_cast<const T*>(p.q) + rows.row_of(m) * p.q_row + head * p.q_head;
+    const T* kb = static_cast<const T*>(p.k) + kv_head * p.k_head;
+    const T* vb = static_cast<const T*>(p.v) + kv_head * p.v_head;
+    float top = -INFINITY, sum = 0.f, o[D / 32];
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) o[i] = 0.f;
+    for (int n0 = lo; n0 < hi; n0 += 32) {
+        const int n = n0 + lane;
+        const int64_t j = t.residue + (int64_t)n * s;
+        const int64_t at = n < hi ? cache_row(p, table, j, p.k_page, p.k_row) : -1;
+        float x = -INFINITY;
+        if (at >= 0) {
+            float dot = 0.f;
+            for (int c = 0; c < p.d; ++c) dot = fmaf(DT<T>::to_f(q[c]), DT<T>::to_f(kb[at + c]), dot);
+            x = (p.softcap > 0.f ? p.softcap * tanhf(dot * p.cap_inv) : dot * p.scale_log2) - slope * (float)(u - n);
+        }
+        const float most = fmaxf(top, warp_max(x)), off = most == -INFINITY ? 0.f : most, corr = exp2f(top - off);
+        const float f = at >= 0 ? exp2f(x - off) : 0.f;
+        sum = sum * corr + f;
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) o[i] *= corr;
+        top = most;
+        for (int k = 0; k < min(32, hi - n0); ++k) {
+            const float fk = __shfl_sync(0xffffffffu, f, k);
+            const int64_t v = cache_row(p, table, t.residue + (int64_t)(n0 + k) * s, p.v_page, p.v_row);
+            if (v < 0) continue;
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i)
+                if (lane + 32 * i < p.d) o[i] = fmaf(fk, DT<T>::to_f(vb[v + lane + 32 * i]), o[i]);
+        }
+    }
+    sum = warp_sum(sum);
+    const int token = (int)rows.row_of(m);
+    if (!whole) {
+        if (lane == 0) p.part_rows[slot] = make_float4(top, sum, __int_as_float(token), __int_as_float(head));
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) p.part_o[slot * D + lane + 32 * i] = o[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i)
+            if (lane + 32 * i < p.d)
+                static_cast<T*>(p.o)[token * p.o_row + head * p.o_head + lane + 32 * i] = DT<T>::from_f(sum != 0.f ? o[i] / sum : 0.f);
+        if (lane == 0 && p.lse != nullptr)
+            p.lse[(int64_t)token * p.kv_heads * (int)p.group.d + head] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
+    }
+}
+
+}  // namespace paged
+}  // namespace splat

@@ -13,6 +13,10 @@
 // tile.  The parts of a tile are added up in the order of its keys: results do not depend on timing, though they do, in the last
 // bits, on what else is in the batch.
 //
+// A tile costs something whatever its length (its rows, its first copies, its end), so it counts for kFixed steps more than it has.  Without
+// that a CTA that came by the short requests of a ragged batch took three times as long as the others: 64 decoding requests of 1 to
+// 16384 tokens (log-uniform), 32 / 8 heads, d128 bf16 249 us without.
+//
 // Steps are counted for a class of a request's longest kind, so that all of its classes and heads have the same tiles; where the count
 // is one too high a CTA has a step without keys.
 #pragma once
@@ -97,12 +101,12 @@ __device__ __forceinline__ int2 steps_of(const Problem& p, const Request& r, int
     const int x = lo / kKeys;
     return make_int2(x, max(x + 1, (hi + kKeys - 1) / kKeys));
 }
-template <int R, int kKeys>
-__device__ __forceinline__ int64_t steps_of_class(const Problem& p, const Request& r) {
+template <int R, int kKeys, int kFixed>
+__device__ __forceinline__ int64_t cost_of_class(const Problem& p, const Request& r) {
     int64_t sum = 0;
     for (int t = 0; t < r.tiles; ++t) {
         const int2 s = steps_of<R, kKeys>(p, r, t);
-        sum += s.y - s.x;
+        sum += s.y - s.x + kFixed;
     }
     return sum;
 }
@@ -111,19 +115,19 @@ __device__ __forceinline__ int64_t divide(int64_t a, int64_t b) {
 }
 
 template <int kThreads> struct WalkShared {
-    int64_t before[kThreads + 1];      // steps in front of a thread's requests
+    int64_t before[kThreads + 1];      // cost in front of a thread's requests
     int64_t warp_sums[kThreads / 32];
 };
 
 // A CTA's walk over its share.  All threads of the block, the same in each.
-template <int R, int kKeys, int kThreads>
+template <int R, int kKeys, int kThreads, int kFixed>
 struct Walk {
-    int64_t at, end;                   // steps, of all
-    int64_t tile_begin;                // of the tile that `at` is in
+    int64_t end;                       // of the share, in steps and fixed costs of all tiles
+    int64_t tile_begin;                // of the tile
+    int64_t at;                        // where the share begins in it: tile_begin, or behind the fixed cost
     int b, head, cls, tile;
     Request r;
     int2 steps;                        // of the tile
-    int64_t class_steps;
 
     // Scans the lengths; false if there is nothing to do for this CTA.
     __device__ bool start(const Problem& p, WalkShared<kThreads>& sh) {
@@ -134,7 +138,7 @@ struct Walk {
             const int q = threadIdx.x * each + i;
             if (q >= p.requests) break;
             const Request x = request_of<R>(p, q);
-            mine += steps_of_class<R, kKeys>(p, x) * x.classes * p.kv_heads;
+            mine += cost_of_class<R, kKeys, kFixed>(p, x) * x.classes * p.kv_heads;
         }
         int64_t x = mine;
 #pragma unroll
@@ -157,36 +161,39 @@ struct Walk {
             const int mid = (lo + hi) >> 1;
             if (sh.before[mid] <= at) lo = mid; else hi = mid;
         }
-        int64_t sum = sh.before[lo];
-        for (b = lo * each;; ++b) {    // (ends: the steps behind `at` are some request's)
+        int64_t sum = sh.before[lo], class_cost;
+        for (b = lo * each;; ++b) {    // (ends: what is behind `at` is some request's)
             r = request_of<R>(p, b);
-            class_steps = steps_of_class<R, kKeys>(p, r);
-            const int64_t w = class_steps * r.classes * p.kv_heads;
+            class_cost = cost_of_class<R, kKeys, kFixed>(p, r);
+            const int64_t w = class_cost * r.classes * p.kv_heads;
             if (at < sum + w) break;
             sum += w;
         }
         int64_t rest = at - sum;
-        const int64_t per_head = class_steps * r.classes;
+        const int64_t per_head = class_cost * r.classes;
         head = (int)divide(rest, per_head);
         rest -= head * per_head;
-        cls = (int)divide(rest, class_steps);
-        rest -= cls * class_steps;
+        cls = (int)divide(rest, class_cost);
+        rest -= cls * class_cost;
         for (tile = 0;; ++tile) {
             steps = steps_of<R, kKeys>(p, r, tile);
-            if (rest < steps.y - steps.x) break;
-            rest -= steps.y - steps.x;
+            if (rest < cost()) break;
+            rest -= cost();
         }
         tile_begin = at - rest;
-        return true;
+        if (rest <= kFixed) at = tile_begin;             // (the whole of it)
+        return end - tile_begin > kFixed || next(p);
     }
-    __device__ __forceinline__ int first_step() const { return steps.x + (int)(at - tile_begin); }
-    __device__ __forceinline__ int last_step() const { return (int)min((int64_t)steps.y, steps.x + (end - tile_begin)); }    // (one behind)
-    __device__ __forceinline__ bool whole() const { return at == tile_begin && end - tile_begin >= steps.y - steps.x; }
-    __device__ __forceinline__ int part() const { return 2 * blockIdx.x + (at == tile_begin ? 1 : 0); }
-    // To the next tile; false at the end of the share.
+    __device__ __forceinline__ int cost() const { return steps.y - steps.x + kFixed; }
+    __device__ __forceinline__ bool begins() const { return at == tile_begin; }
+    __device__ __forceinline__ int first_step() const { return begins() ? steps.x : steps.x + (int)(at - tile_begin) - kFixed; }
+    __device__ __forceinline__ int last_step() const { return (int)min((int64_t)steps.y, steps.x + (end - tile_begin - kFixed)); }    // (one behind)
+    __device__ __forceinline__ bool whole() const { return begins() && end - tile_begin >= cost(); }
+    __device__ __forceinline__ int part() const { return 2 * blockIdx.x + (begins() ? 1 : 0); }
+    // To the next tile; false at the end of the share: a tile of which no step is left in it is the next CTA's.
     __device__ bool next(const Problem& p) {
-        at = tile_begin + (steps.y - steps.x);
-        if (at >= end) return false;
+        at = tile_begin + cost();
+        if (end - at <= kFixed) return false;
         tile_begin = at;
         if (++tile == r.tiles) {
             tile = 0;
@@ -208,7 +215,7 @@ struct TileRows {
     int count;                         // tokens of the class
     int u0;                            // index of its first among the class's keys
     int residue;                       // key n of the class is token residue + n * stride
-    template <int R, int K, int N> __device__ __forceinline__ static TileRows of(const Problem& p, const Walk<R, K, N>& w) {
+    template <int R, int K, int N, int F> __device__ __forceinline__ static TileRows of(const Problem& p, const Walk<R, K, N, F>& w) {
         TileRows t;
         const int s = (int)p.stride.d, pos = w.r.pos + w.cls;
         t.count = p.stride.div(w.r.n - w.cls + s - 1);
