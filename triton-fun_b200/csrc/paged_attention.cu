@@ -385,9 +385,17 @@ bool cache_map(CUtensorMap* map, const splat_paged_args& a, const void* base, in
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// paged_decode.cu
+// paged_decode.cu, paged_chunk.cu (which may answer SPLAT_ERR_UNSUPPORTED_SHAPE, and has then launched nothing)
 int decode_ctas(int sms);
 int32_t attend_decode(const splat_paged_args& a, Problem p, int sms, void* workspace, cudaStream_t st);
+int chunk_ctas(int sms);
+int32_t attend_chunk(const splat_paged_args& a, Problem p, int sms, void* workspace, cudaStream_t st);
+constexpr int kFewRows = 16;           // rows of a request's class up to which paged_decode.cu takes it
+// most rows that a request's class can have
+static int64_t chunk_rows(const splat_paged_args& a) {
+    const int64_t n = a.max_q_len < a.tokens ? a.max_q_len : a.tokens;
+    return (n / a.stride + (n % a.stride != 0)) * (a.heads / a.kv_heads);
+}
 
 }  // namespace paged
 }  // namespace splat
@@ -396,7 +404,10 @@ extern "C" int64_t splat_paged_attention_workspace(const splat_paged_args* a) {
     using namespace splat::paged;
     if (!a || check_args(*a) != SPLAT_OK) return 0;
     const int sms = sm_count();
-    if (tensor_cores(*a)) return Layout(decode_ctas(sms), 16, d_pad_any(a->d)).bytes;
+    if (tensor_cores(*a)) {
+        const int64_t few = Layout(decode_ctas(sms), 16, d_pad_any(a->d)).bytes, many = Layout(chunk_ctas(sms), 128, d_pad_any(a->d)).bytes;
+        return chunk_rows(*a) > kFewRows && many > few ? many : few;
+    }
     return Layout(sms * kPerSmAny, kRowsAny, d_pad_any(a->d)).bytes;
 }
 
@@ -435,7 +446,21 @@ extern "C" int32_t splat_paged_attention(const splat_paged_args* args, void* str
     const int ctas = sms * kPerSmAny;
     p.rows_from = 0;
     p.rows_to = INT32_MAX;
-    if (tensor_cores(a)) return attend_decode(a, p, sms, a.workspace, st);
+    if (tensor_cores(a)) {
+        // Requests of few rows and of many, one after the other where there may be both; they share the workspace, which is why the
+        // second waits for the joining of the first
+        if (chunk_rows(a) > kFewRows) {
+            const bool alike = a.tokens == a.requests * a.max_q_len;           // as a rule: all of them bring as many
+            p.rows_from = alike ? 0 : kFewRows + 1;
+            const int32_t rc = attend_chunk(a, p, sms, a.workspace, st);
+            if (rc != SPLAT_ERR_UNSUPPORTED_SHAPE) {
+                if (rc != SPLAT_OK || alike) return rc;
+                p.rows_to = kFewRows;
+            }
+            p.rows_from = 0;
+        }
+        return attend_decode(a, p, sms, a.workspace, st);
+    }
     if (a.dtype == SPLAT_F32) return launch_any<float>(a, p, ctas, st);
     if (a.dtype == SPLAT_F16) return launch_any<__half>(a, p, ctas, st);
     return launch_any<__nv_bfloat16>(a, p, ctas, st);

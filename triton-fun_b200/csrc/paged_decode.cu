@@ -396,7 +396,14 @@ paged_decode_kernel(const __grid_constant__ Maps maps, const __grid_constant__ P
         __syncthreads();
         if (odd_rows != 0) {                                           // perhaps by keys that the row does not see: from its own alone
             for (int r = warp; r < kRows; r += kWarps)
-                if ((odd_rows >> r) & 1u) row_again<T, D>(p, w.head, table, t, rows, r, lo, hi, whole, part * kRows + r);
+                if ((odd_rows >> r) & 1u) {
+                    const int m = rows.token_of(r);
+                    RowKeys x;
+                    x.table = table; x.slot = part * kRows + r; x.whole = whole;
+                    x.token = (int)rows.row_of(m); x.head = rows.head_of(r, m); x.kv_head = w.head; x.residue = t.residue;
+                    x.u = t.u0 + m; x.lo = max(lo, x.u - p.taps + 1); x.hi = min(hi, x.u + 1);
+                    row_again<T, D>(p, x);
+                }
             __syncthreads();
         }
         if (kTma) {

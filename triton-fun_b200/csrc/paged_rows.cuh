@@ -77,41 +77,43 @@ __device__ __forceinline__ void put_row(const Problem& p, bool whole, int64_t sl
         p.lse[(int64_t)token * p.kv_heads * (int)p.group.d + head] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
 }
 
-// Row r of the tile over its own keys in [lo, hi), by one warp.  A tile multiplies keys that a row does not see with probability 0, and 0
+// A row over its own keys [lo, hi) of a class, by one warp.  A tile multiplies keys that a row does not see with probability 0, and 0
 // times infinity is NaN; such rows are rare, are noticed at the end, and come here.
-template <typename T, int D, int R>
-__device__ __noinline__ void row_again(const Problem& p, int kv_head, const int32_t* table, const TileRows t, const RowPlace<R> rows, int r, int lo,
-                                       int hi, bool whole, int64_t slot) {
+struct RowKeys {
+    const int32_t* table;
+    int64_t slot;                      // of the parts, unless `whole`
+    int token, head, kv_head, residue, u, lo, hi;
+    bool whole;
+};
+template <typename T, int D>
+__device__ __noinline__ void row_again(const Problem& p, const RowKeys& x) {
     const int lane = threadIdx.x & 31, s = (int)p.stride.d;
-    const int m = rows.token_of(r), head = rows.head_of(r, m), u = t.u0 + m;
-    lo = max(lo, u - p.taps + 1);
-    hi = min(hi, u + 1);
-    const float slope = p.slopes != nullptr ? p.slopes[head] * kLog2e * (float)s : 0.f;
-    const T* q = static_cast<const T*>(p.q) + rows.row_of(m) * p.q_row + head * p.q_head;
-    const T* kb = static_cast<const T*>(p.k) + kv_head * p.k_head;
-    const T* vb = static_cast<const T*>(p.v) + kv_head * p.v_head;
+    const float slope = p.slopes != nullptr ? p.slopes[x.head] * kLog2e * (float)s : 0.f;
+    const T* q = static_cast<const T*>(p.q) + x.token * p.q_row + x.head * p.q_head;
+    const T* kb = static_cast<const T*>(p.k) + x.kv_head * p.k_head;
+    const T* vb = static_cast<const T*>(p.v) + x.kv_head * p.v_head;
     float top = -INFINITY, sum = 0.f, o[D / 32];
 #pragma unroll
     for (int i = 0; i < D / 32; ++i) o[i] = 0.f;
-    for (int n0 = lo; n0 < hi; n0 += 32) {
+    for (int n0 = x.lo; n0 < x.hi; n0 += 32) {
         const int n = n0 + lane;
-        const int64_t j = t.residue + (int64_t)n * s;
-        const int64_t at = n < hi ? cache_row(p, table, j, p.k_page, p.k_row) : -1;
-        float x = -INFINITY;
+        const int64_t j = x.residue + (int64_t)n * s;
+        const int64_t at = n < x.hi ? cache_row(p, x.table, j, p.k_page, p.k_row) : -1;
+        float y = -INFINITY;
         if (at >= 0) {
             float dot = 0.f;
             for (int c = 0; c < p.d; ++c) dot = fmaf(DT<T>::to_f(q[c]), DT<T>::to_f(kb[at + c]), dot);
-            x = (p.softcap > 0.f ? p.softcap * tanhf(dot * p.cap_inv) : dot * p.scale_log2) - slope * (float)(u - n);
+            y = (p.softcap > 0.f ? p.softcap * tanhf(dot * p.cap_inv) : dot * p.scale_log2) - slope * (float)(x.u - n);
         }
-        const float most = fmaxf(top, warp_max(x)), off = most == -INFINITY ? 0.f : most, corr = exp2f(top - off);
-        const float f = at >= 0 ? exp2f(x - off) : 0.f;
+        const float most = fmaxf(top, warp_max(y)), off = most == -INFINITY ? 0.f : most, corr = exp2f(top - off);
+        const float f = at >= 0 ? exp2f(y - off) : 0.f;
         sum = sum * corr + f;
 #pragma unroll
         for (int i = 0; i < D / 32; ++i) o[i] *= corr;
         top = most;
-        for (int k = 0; k < min(32, hi - n0); ++k) {
+        for (int k = 0; k < min(32, x.hi - n0); ++k) {
             const float fk = __shfl_sync(0xffffffffu, f, k);
-            const int64_t v = cache_row(p, table, t.residue + (int64_t)(n0 + k) * s, p.v_page, p.v_row);
+            const int64_t v = cache_row(p, x.table, x.residue + (int64_t)(n0 + k) * s, p.v_page, p.v_row);
             if (v < 0) continue;
 #pragma unroll
             for (int i = 0; i < D / 32; ++i)
@@ -119,18 +121,18 @@ __device__ __noinline__ void row_again(const Problem& p, int kv_head, const int3
         }
     }
     sum = warp_sum(sum);
-    const int token = (int)rows.row_of(m);
-    if (!whole) {
-        if (lane == 0) p.part_rows[slot] = make_float4(top, sum, __int_as_float(token), __int_as_float(head));
+    __syncwarp();                      // (what the tile wrote of the row stands before this)
+    if (!x.whole) {
+        if (lane == 0) p.part_rows[x.slot] = make_float4(top, sum, __int_as_float(x.token), __int_as_float(x.head));
 #pragma unroll
-        for (int i = 0; i < D / 32; ++i) p.part_o[slot * D + lane + 32 * i] = o[i];
+        for (int i = 0; i < D / 32; ++i) p.part_o[x.slot * D + lane + 32 * i] = o[i];
     } else {
 #pragma unroll
         for (int i = 0; i < D / 32; ++i)
             if (lane + 32 * i < p.d)
-                static_cast<T*>(p.o)[token * p.o_row + head * p.o_head + lane + 32 * i] = DT<T>::from_f(sum != 0.f ? o[i] / sum : 0.f);
+                static_cast<T*>(p.o)[x.token * p.o_row + x.head * p.o_head + lane + 32 * i] = DT<T>::from_f(sum != 0.f ? o[i] / sum : 0.f);
         if (lane == 0 && p.lse != nullptr)
-            p.lse[(int64_t)token * p.kv_heads * (int)p.group.d + head] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
+            p.lse[(int64_t)x.token * p.kv_heads * (int)p.group.d + x.head] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
     }
 }
 
