@@ -21,36 +21,8 @@ def rrotary_launcher(q: torch.Tensor, k, positions: torch.Tensor, inv_freq: torc
     return _n.rotary(q, k, positions, inv_freq, sections, interleaved, inverse, q_out, k_out)
 
 
-class _Rotary(torch.autograd.Function):
-    """The gradient of a rotation is the rotation by the opposite angle."""
-
-    @staticmethod
-    def forward(ctx, q, k, positions, inv_freq, sections, interleaved, inverse):
-        ctx.set_materialize_grads(False)
-        ctx.save_for_backward(positions, inv_freq)
-        ctx.how = sections, interleaved, inverse
-        return _n.rotary(q, k, positions, inv_freq, sections, interleaved, inverse, None, None)
-
-    @staticmethod
-    def backward(ctx, dq, dk):
-        positions, inv_freq = ctx.saved_tensors
-        sections, interleaved, inverse = ctx.how
-        wanted = [g if need and g is not None else None for g, need in zip((dq, dk), ctx.needs_input_grad)]
-        # (a gradient may come expanded, as that of a sum)
-        rows = [g if g is None or g.stride(-1) == 1 else g.contiguous() for g in wanted]
-        first, second = (rows[0], rows[1]) if rows[0] is not None else (rows[1], None)
-        if first is None:
-            return (None,) * 7
-        a, b = _Rotary.apply(first, second, positions, inv_freq, sections, interleaved, not inverse)
-        return (*((a, b) if rows[0] is not None else (None, a)), None, None, None, None, None)
-
-
 def rrotary(q: torch.Tensor, k, positions: torch.Tensor, inv_freq: torch.Tensor, sections=None, *,
             interleaved: bool = False):
-    """``rrotary_launcher`` into new tensors, differentiable in q and k (also twice): (q', k'), k' None without k."""
-    if torch.is_grad_enabled():
-        if inv_freq.requires_grad:
-            raise ValueError("inv_freq must not require a gradient: there is none for the frequencies")
-        if q.requires_grad or (k is not None and k.requires_grad):
-            return _Rotary.apply(q, k, positions, inv_freq, sections, interleaved, False)
-    return _n.rotary(q, k, positions, inv_freq, sections, interleaved, False, None, None)
+    """``rrotary_launcher`` into new tensors, differentiable in q and k (also twice): (q', k'), k' None without k.  The
+    gradient of a rotation is the rotation by the opposite angle, one launch for both."""
+    return _n.rotary_grad(q, k, positions, inv_freq, sections, interleaved)

@@ -677,4 +677,4 @@ _host.bind_paged(*(ctypes.cast(getattr(_lib, name), _vp).value for name in (
     "splat_paged_tables", "splat_rotary", "splat_paged_attention_workspace", "splat_paged_attention",
     "splat_status_string")), _prepare_paged)
 paged_tables, paged_append, paged_attention = _host.paged_tables, _host.paged_append, _host.paged_attention
-rotary = _host.rotary
+rotary, rotary_grad = _host.rotary, _host.rotary_grad

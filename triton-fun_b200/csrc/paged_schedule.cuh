@@ -22,21 +22,10 @@
 #pragma once
 
 #include "common.cuh"
+#include "fast_div.cuh"
 
 namespace splat {
 namespace paged {
-
-struct FastDiv {               // n / d for 0 <= n < 2^31
-    uint32_t mul, shift, d;
-    FastDiv() = default;
-    explicit FastDiv(uint32_t d_) : d(d_) {
-        shift = 0;
-        while ((1ull << shift) < d) ++shift;
-        mul = (uint32_t)(((1ull << 32) * ((1ull << shift) - d)) / d + 1);
-    }
-    __device__ __forceinline__ int div(int n) const { return (int)((__umulhi(mul, (uint32_t)n) + (uint32_t)n) >> shift); }
-    __device__ __forceinline__ int div_floor(int n) const { return n >= 0 ? div(n) : -1 - div(-1 - n); }
-};
 
 constexpr int kMaxLen = 1 << 30;       // of a request, in tokens
 constexpr int kAllTaps = 1 << 30;

@@ -7,19 +7,25 @@
 // with a, b = elements i and i + half, or 2 i and 2 i + 1 where pairs lie side by side.  axis(i): the first sections[0] pairs go
 // by axis 0, the next sections[1] by axis 1, and so on.  Elements behind the turned ones are copied.
 //
-// Every element is read once and written once, and that is what bounds it.  A thread keeps one unit of pairs (as many as fill 16
-// bytes) of one token and walks over heads, so that the angles' cosines and sines are found once and stay in registers.  How many
-// heads a thread walks over goes by the size of the call: all of them in a large one (16 pairs of double precision for 64 heads), few
-// in a small one, where the heads' latencies would follow one another.
+// Every element is read once and written once, and that is what bounds it.  A block takes a few tokens and several groups of heads; the
+// tokens' cosines and sines are found once, in shared memory (by every thread that needs them they are three and more times as many, and
+// 15 million cost 75 us).  A thread has one unit of pairs (as many as fill 16 bytes) of one token and two or four heads, whose pieces are
+// all requested at its start and arrive while the angles are formed.  Small blocks, many to an SM, so that some copy while others
+// compute.  us, bf16 B2 H32+32 L4096 d128 with three axes / fp16 append of 8191 tokens, H16+16+16 d64: blocks of 256 threads with eight
+// heads each, two to an SM 59.8 / 28.1; four heads, four to an SM 55.8 / 25.8; 128 threads with four heads, six to an SM 48.7 / 22.4,
+// eight 46.4 / 21.5 (5.8 TB/s / 4.7 TB/s); 64 threads, sixteen 46.3 / 24.8; torch's copies of the first 49.2.  Angles formed by
+// every thread, walking over 22 heads: 69 / 23.
 //
 // The angle is formed in turns, in 64 bits: position times frequency of a far token has more than the 24 bits of fp32 in front
 // of its fraction.  cos and sin are of the fraction, in fp32, as are the products; they are rounded once, to the result's type.
 #include "common.cuh"
+#include "fast_div.cuh"
 
 namespace splat {
 namespace rotary {
 
-constexpr int kThreads = 128;
+constexpr int kThreads = 128, kPerSm = 8;     // (64 registers)
+constexpr int kHeads = 4;                      // most heads of a thread, all requested at once
 constexpr int kMaxRows = 3;                    // arrays of rows in a call: q and k, or q, k and v
 
 struct Args {
@@ -36,8 +42,10 @@ struct Args {
     int d;
     const int64_t* slots;                      // (B * L): row of the paged cache, for rows with `paged`
     int64_t page, slots_end;
-    int heads_per_thread;
     int units, turned_units;                   // of a row: units of pairs first, then single pieces that are copied
+    int tokens, groups, group_heads;           // of a block: tokens, and groups of heads
+    int block_units;
+    FastDiv length_div, half_div, page_div;
 };
 
 template <typename T, int V> struct Piece;     // V elements
@@ -58,80 +66,109 @@ template <typename T, int V> struct Piece {
     __device__ __forceinline__ void set(int i, float v) { x[i] = DT<T>::from_f(v); }
 };
 
+// The unit's pairs in x and y, by the angles of cs and sn
 template <typename T, int V>
-__global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant__ Args a) {
+__device__ __forceinline__ void turn_pairs(Piece<T, V>& x, Piece<T, V>& y, const float (&cs)[V], const float (&sn)[V], bool side_by_side) {
+    if (V > 1 && side_by_side) {                           // the first half of the pairs in x, the others in y
+#pragma unroll
+        for (int i = 0; i < V; i += 2) {
+            const float p0 = x.get(i), p1 = x.get(i + (V > 1)), q0 = y.get(i), q1 = y.get(i + (V > 1));
+            const int j = i / 2, k = V / 2 + i / 2;
+            x.set(i, p0 * cs[j] - p1 * sn[j]);
+            x.set(i + (V > 1), p0 * sn[j] + p1 * cs[j]);
+            y.set(i, q0 * cs[k] - q1 * sn[k]);
+            y.set(i + (V > 1), q0 * sn[k] + q1 * cs[k]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const float p0 = x.get(i), p1 = y.get(i);
+            x.set(i, p0 * cs[i] - p1 * sn[i]);
+            y.set(i, p0 * sn[i] + p1 * cs[i]);
+        }
+    }
+}
+
+// A head's place in its array
+template <typename T> struct Head {
+    const T* src;
+    T* dst;
+    bool turn, to;
+    __device__ __forceinline__ Head(const Args& a, int h, int b, int l, int slot_page, int slot_row) {
+        int r = 0;
+        while (r + 1 < a.n_rows && h >= (int)a.rows[r].heads) h -= (int)a.rows[r++].heads;
+        const splat_rows& x = a.rows[r];
+        src = static_cast<const T*>(x.src) + b * x.src_b + l * x.src_l + h * x.src_h;
+        dst = static_cast<T*>(x.dst) + (x.paged ? slot_page : b) * x.dst_b + (x.paged ? slot_row : l) * x.dst_l + h * x.dst_h;
+        turn = x.turned;
+        to = !x.paged || slot_page >= 0;
+    }
+};
+
+template <typename T, int V>
+__global__ void __launch_bounds__(kThreads, kPerSm) rotary_kernel(const __grid_constant__ Args a) {
+    extern __shared__ float2 angles[];                         // cosine and sine, [token of the block][pair]
     depend_wait();
     depend_release();
-    const int64_t id = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-    const int64_t token = id / a.units;
-    const int unit = (int)(id - token * a.units);
-    if (token >= a.batch * a.length) return;
-    const int64_t b = token / a.length, l = token - b * a.length;
+    const int first = (int)blockIdx.x * a.tokens, all = (int)(a.batch * a.length);
+    const int unit = (int)(threadIdx.x % a.block_units + blockIdx.z * a.block_units), at = threadIdx.x / a.block_units % a.tokens;
+    const int token = first + at;
+    int h = ((int)blockIdx.y * a.groups + (int)threadIdx.x / (a.tokens * a.block_units)) * a.group_heads;
+    const int h_end = token < all && unit < a.units && (int)threadIdx.x < a.tokens * a.block_units * a.groups ? min(h + a.group_heads, a.heads) : 0;
+    const int b = a.length_div.div(token), l = token - b * (int)a.length_div.d;
     const bool turned = unit < a.turned_units;
     // where the unit's two pieces begin in a row; a unit behind the turned pairs has one
     const int at0 = turned ? unit * V * (a.interleaved ? 2 : 1) : 2 * a.half + (unit - a.turned_units) * V;
     const int at1 = a.interleaved ? at0 + V : at0 + a.half;
+    int slot_page = -1, slot_row = 0;
+    if (a.slots != nullptr && h < h_end) {
+        const int64_t slot = __ldg(a.slots + token);
+        if (slot >= 0 && slot < a.slots_end) {
+            slot_page = a.page_div.div((int)slot);
+            slot_row = (int)slot - slot_page * (int)a.page_div.d;
+        }
+    }
+    Piece<T, V> x[kHeads], y[kHeads];                          // (on their way while the angles are formed)
+#pragma unroll
+    for (int k = 0; k < kHeads; ++k)
+        if (h + k < h_end) {
+            const Head<T> head(a, h + k, b, l, slot_page, slot_row);
+            x[k].load(head.src + at0);
+            if (turned) y[k].load(head.src + at1);
+        }
+    for (int i = threadIdx.x; i < a.tokens * a.half; i += blockDim.x) {
+        const int row = a.half_div.div(i), pair = i - row * a.half;
+        if (first + row >= all) break;
+        int axis = 0;
+        while (axis + 1 < a.axes && pair >= a.section_end[axis]) ++axis;
+        const int pb = a.length_div.div(first + row), pl = first + row - pb * (int)a.length_div.d;
+        const int64_t where = axis * a.pos_axis + pb * a.pos_b + pl * a.pos_l;
+        const int64_t pos = a.positions_64 ? static_cast<const int64_t*>(a.positions)[where] : static_cast<const int32_t*>(a.positions)[where];
+        const double turns = (double)pos * (double)__ldg(a.inv_freq + pair) * 0.15915494309189533577;      // 1 / 2 pi
+        float2 cs;
+        sincospif((float)(2.0 * (turns - rint(turns))), &cs.y, &cs.x);
+        if (a.inverse) cs.y = -cs.y;
+        angles[i] = cs;
+    }
+    __syncthreads();
     float cs[V], sn[V];
-    if (turned) {
+    if (turned && h < h_end) {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            const int pair = unit * V + i;
-            int axis = 0;
-            while (axis + 1 < a.axes && pair >= a.section_end[axis]) ++axis;
-            const int64_t where = axis * a.pos_axis + b * a.pos_b + l * a.pos_l;
-            const int64_t pos = a.positions_64 ? static_cast<const int64_t*>(a.positions)[where] : static_cast<const int32_t*>(a.positions)[where];
-            const double turns = (double)pos * (double)__ldg(a.inv_freq + pair) * 0.15915494309189533577;
-            sincospif((float)(2.0 * (turns - rint(turns))), &sn[i], &cs[i]);
-            if (a.inverse) sn[i] = -sn[i];
+            const float2 c = angles[at * a.half + unit * V + i];
+            cs[i] = c.x;
+            sn[i] = c.y;
         }
     }
-    int64_t slot = -1;
-    if (a.slots != nullptr) slot = a.slots[token];
-    const int64_t slot_page = slot >= 0 && slot < a.slots_end ? slot / a.page : -1;
-    const int64_t slot_row = slot - slot_page * a.page;
-
-    int h = blockIdx.y * a.heads_per_thread;
-    const int h_end = min(h + a.heads_per_thread, a.heads);
-    int base = 0;                                          // heads of the arrays in front
-    for (int r = 0; r < a.n_rows; base += (int)a.rows[r].heads, ++r) {
-        const splat_rows& rows = a.rows[r];
-        const int end = min(h_end, base + (int)rows.heads);
-        if (h >= end) continue;
-        const int64_t dst_b = rows.paged ? slot_page : b, dst_l = rows.paged ? slot_row : l;
-        const bool to = !rows.paged || slot_page >= 0;
-        const T* src = static_cast<const T*>(rows.src) + b * rows.src_b + l * rows.src_l + (h - base) * rows.src_h;
-        T* dst = static_cast<T*>(rows.dst) + dst_b * rows.dst_b + dst_l * rows.dst_l + (h - base) * rows.dst_h;
-        const bool turn = turned && rows.turned;
-        if (!to) { h = end; continue; }
-#pragma unroll 4
-        for (; h < end; ++h, src += rows.src_h, dst += rows.dst_h) {
-            Piece<T, V> x, y;
-            x.load(src + at0);
-            if (turned) y.load(src + at1);
-            if (turn) {
-                if (V > 1 && a.interleaved) {              // pairs side by side: the first half of them in x, the others in y
 #pragma unroll
-                    for (int i = 0; i < V; i += 2) {
-                        const float p0 = x.get(i), p1 = x.get(i + (V > 1)), q0 = y.get(i), q1 = y.get(i + (V > 1));
-                        const int j = i / 2, k = V / 2 + i / 2;
-                        x.set(i, p0 * cs[j] - p1 * sn[j]);
-                        x.set(i + (V > 1), p0 * sn[j] + p1 * cs[j]);
-                        y.set(i, q0 * cs[k] - q1 * sn[k]);
-                        y.set(i + (V > 1), q0 * sn[k] + q1 * cs[k]);
-                    }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < V; ++i) {
-                        const float p0 = x.get(i), p1 = y.get(i);
-                        x.set(i, p0 * cs[i] - p1 * sn[i]);
-                        y.set(i, p0 * sn[i] + p1 * cs[i]);
-                    }
-                }
-            }
-            x.store(dst + at0);
-            if (turned) y.store(dst + at1);
+    for (int k = 0; k < kHeads; ++k)
+        if (h + k < h_end) {
+            const Head<T> head(a, h + k, b, l, slot_page, slot_row);
+            if (!head.to) continue;
+            if (turned && head.turn) turn_pairs<T, V>(x[k], y[k], cs, sn, a.interleaved);
+            x[k].store(head.dst + at0);
+            if (turned) y[k].store(head.dst + at1);
         }
-    }
 }
 
 template <typename T>
@@ -147,15 +184,25 @@ int32_t launch(Args& a, cudaStream_t st) {
     const int v = wide ? V : 1;
     a.turned_units = a.half / v;
     a.units = a.turned_units + (a.d - 2 * a.half) / v;
-    const int64_t threads = a.batch * a.length * a.units, blocks = (threads + kThreads - 1) / kThreads;
-    if (blocks > INT32_MAX) return SPLAT_ERR_UNSUPPORTED_SHAPE;
-    // As many threads as keep the GPU's memory busy (148 SMs with 1024 threads), then heads one after another
-    const int64_t splits = (148 * 1024 + threads - 1) / threads;
-    a.heads_per_thread = (int)(splits >= a.heads ? 1 : (a.heads + splits - 1) / splits);
-    const int64_t y = (a.heads + a.heads_per_thread - 1) / a.heads_per_thread;
-    if (y > 65535) return SPLAT_ERR_UNSUPPORTED_SHAPE;
-    const dim3 grid((unsigned)blocks, (unsigned)y);
-    return wide ? launch_kernel(rotary_kernel<T, V>, grid, dim3(kThreads), 0, st, a) : launch_kernel(rotary_kernel<T, 1>, grid, dim3(kThreads), 0, st, a);
+    const int64_t all = a.batch * a.length;
+    if (all > INT32_MAX || a.slots_end > INT32_MAX || a.length > INT32_MAX) return SPLAT_ERR_UNSUPPORTED_SHAPE;
+    // Heads of a thread: four in calls that fill the GPU (148 SMs with 1024 threads) twice over, else two (fp32 B3 H12+4 L1369 d64: 5.7 us, 8.3 with four)
+    a.group_heads = all * a.units * a.heads >= (int64_t)8 * 148 * 1024 ? kHeads : 2;
+    const int groups = (a.heads + a.group_heads - 1) / a.group_heads;
+    a.block_units = a.units < kThreads ? a.units : kThreads;
+    const int fit = kThreads / a.block_units;                  // groups of heads, or tokens
+    a.groups = fit < groups ? fit : groups;
+    a.tokens = kThreads / (a.block_units * a.groups);
+    const int threads = (a.tokens * a.block_units * a.groups + 31) / 32 * 32;
+    a.length_div = FastDiv((uint32_t)a.length);
+    a.half_div = FastDiv((uint32_t)(a.half > 0 ? a.half : 1));
+    a.page_div = FastDiv((uint32_t)a.page);
+    const int64_t x = (all + a.tokens - 1) / a.tokens, y = (groups + a.groups - 1) / a.groups, z = (a.units + a.block_units - 1) / a.block_units;
+    const int64_t bytes = (int64_t)a.tokens * a.half * 8;
+    if (y > 65535 || z > 65535 || bytes > 48 * 1024) return SPLAT_ERR_UNSUPPORTED_SHAPE;
+    const dim3 grid((unsigned)x, (unsigned)y, (unsigned)z);
+    return wide ? launch_kernel(rotary_kernel<T, V>, grid, dim3(threads), (size_t)bytes, st, a)
+                : launch_kernel(rotary_kernel<T, 1>, grid, dim3(threads), (size_t)bytes, st, a);
 }
 
 }  // namespace rotary
