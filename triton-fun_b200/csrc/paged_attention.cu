@@ -231,66 +231,85 @@ template <typename T, int kD>
 __global__ void __launch_bounds__(kThreadsJoin) paged_join_kernel(const Problem p, const int ctas, const int rows) {
     constexpr int kEach = (kD + 127) / 128;                // pieces of 4 columns of a lane
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = blockIdx.x + 1;
+    const int r = blockIdx.y * (kThreadsJoin / 32) + warp;
     depend_wait();
     depend_release();
-    const int64_t id = p.begins[c];
-    if (id < 0 || p.begins[c - 1] == id) return;
-    int n = 1;                                             // parts
-    for (int j = c; j < ctas; j += 32) {
-        const unsigned same = __ballot_sync(0xffffffffu, j + lane < ctas && p.begins[min(j + lane, ctas - 1)] == id);
-        n += __popc(same);
-        if (same != 0xffffffffu) break;
+    // One look at the CTA's neighbours: c - 1, c, c + 1, ... by lane
+    const int64_t seen = c - 1 + lane < ctas ? p.begins[c - 1 + lane] : -1;
+    const int64_t id = __shfl_sync(0xffffffffu, seen, 1);
+    if (id < 0 || __shfl_sync(0xffffffffu, seen, 0) == id || r >= rows) return;
+    const unsigned same = __ballot_sync(0xffffffffu, seen == id) >> 1;
+    int n = 1 + __ffs(~same) - 1;                          // parts
+    for (int j = c + 31; n == 32 + j - c - 31 && j < ctas; j += 32) {      // (more than 31 CTAs begin in the middle of the tile)
+        const unsigned more = __ballot_sync(0xffffffffu, j + lane < ctas && p.begins[min(j + lane, ctas - 1)] == id);
+        n += more == 0xffffffffu ? 32 : __ffs(~more) - 1;
+        if (more != 0xffffffffu) break;
     }
-    auto part = [&](int i) { return (int64_t)(i == 0 ? 2 * (c - 1) + 1 : 2 * (c - 1 + i)); };
-    for (int r = blockIdx.y * (kThreadsJoin / 32) + warp; r < rows; r += gridDim.y * (kThreadsJoin / 32)) {
-        const float4 first = p.part_rows[part(0) * rows + r];
-        const int token = __float_as_int(first.z), head = __float_as_int(first.w);
-        if (token < 0) continue;
-        float most = -INFINITY;
-        for (int i = lane; i < n; i += 32) most = fmaxf(most, p.part_rows[part(i) * rows + r].x);
-        most = warp_max(most);
-        const float base = most == -INFINITY ? 0.f : most;
-        float all = 0.f, o[kEach][4];
+    auto part = [&](int i) { return (int64_t)(i == 0 ? 2 * (c - 1) + 1 : 2 * (c - 1 + i)) * rows + r; };
+    // The first parts' columns are requested together with the maxima and sums
+    constexpr int kAhead = 4;
+    float4 x[kAhead][kEach];
 #pragma unroll
-        for (int e = 0; e < kEach; ++e)
+    for (int i = 0; i < kAhead; ++i)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) o[e][k] = 0.f;
-        for (int i0 = 0; i0 < n; i0 += 32) {
-            float f = 0.f;
-            if (i0 + lane < n) {
-                const float4 x = p.part_rows[part(i0 + lane) * rows + r];
-                f = exp2f(x.x - base);
-                all += f * x.y;
-            }
-            const int here = min(32, n - i0);
-#pragma unroll 8
-            for (int i = 0; i < here; ++i) {
+        for (int e = 0; e < kEach; ++e) {
+            const int col = e * 128 + lane * 4;
+            x[i][e] = i < n && col < kD ? *reinterpret_cast<const float4*>(p.part_o + part(i) * kD + col) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+    float4 mine = lane < n ? p.part_rows[part(lane)] : make_float4(-INFINITY, 0.f, 0.f, 0.f);
+    const int token = __float_as_int(__shfl_sync(0xffffffffu, mine.z, 0)), head = __float_as_int(__shfl_sync(0xffffffffu, mine.w, 0));
+    if (token < 0) return;
+    float most = mine.x;
+    for (int i = 32 + lane; i < n; i += 32) most = fmaxf(most, p.part_rows[part(i)].x);
+    most = warp_max(most);
+    const float base = most == -INFINITY ? 0.f : most;
+    float all = 0.f, o[kEach][4];
+#pragma unroll
+    for (int e = 0; e < kEach; ++e)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) o[e][k] = 0.f;
+    auto add = [&](float f, const float4& y, int e) {
+        o[e][0] = fmaf(f, y.x, o[e][0]);
+        o[e][1] = fmaf(f, y.y, o[e][1]);
+        o[e][2] = fmaf(f, y.z, o[e][2]);
+        o[e][3] = fmaf(f, y.w, o[e][3]);
+    };
+    for (int i0 = 0; i0 < n; i0 += 32) {
+        if (i0 > 0) mine = i0 + lane < n ? p.part_rows[part(i0 + lane)] : make_float4(-INFINITY, 0.f, 0.f, 0.f);
+        const float f = exp2f(mine.x - base);
+        all = fmaf(f, mine.y, all);
+        const int here = min(32, n - i0);
+        int i = 0;
+        if (i0 == 0) {
+#pragma unroll
+            for (; i < kAhead; ++i) {
                 const float fi = __shfl_sync(0xffffffffu, f, i);
+                if (i < n)
 #pragma unroll
-                for (int e = 0; e < kEach; ++e) {
-                    const int col = e * 128 + lane * 4;
-                    if (col < kD) {
-                        const float4 x = *reinterpret_cast<const float4*>(p.part_o + (part(i0 + i) * rows + r) * kD + col);
-                        o[e][0] = fmaf(fi, x.x, o[e][0]);
-                        o[e][1] = fmaf(fi, x.y, o[e][1]);
-                        o[e][2] = fmaf(fi, x.z, o[e][2]);
-                        o[e][3] = fmaf(fi, x.w, o[e][3]);
-                    }
-                }
+                    for (int e = 0; e < kEach; ++e) add(fi, x[i][e], e);
             }
         }
-        all = warp_sum(all);
-        T* out = static_cast<T*>(p.o) + token * p.o_row + head * p.o_head;
+#pragma unroll 8
+        for (; i < here; ++i) {
+            const float fi = __shfl_sync(0xffffffffu, f, i);
 #pragma unroll
-        for (int e = 0; e < kEach; ++e)
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int col = e * 128 + lane * 4 + k;
-                if (col < p.d) out[col] = DT<T>::from_f(all != 0.f ? o[e][k] / all : 0.f);
+            for (int e = 0; e < kEach; ++e) {
+                const int col = e * 128 + lane * 4;
+                if (col < kD) add(fi, *reinterpret_cast<const float4*>(p.part_o + part(i0 + i) * kD + col), e);
             }
-        if (lane == 0 && p.lse != nullptr)
-            p.lse[(int64_t)token * p.kv_heads * (int)p.group.d + head] = all == 0.f ? -INFINITY : (most + log2f(all)) * kLn2;
+        }
     }
+    all = warp_sum(all);
+    T* out = static_cast<T*>(p.o) + token * p.o_row + head * p.o_head;
+#pragma unroll
+    for (int e = 0; e < kEach; ++e)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int col = e * 128 + lane * 4 + k;
+            if (col < p.d) out[col] = DT<T>::from_f(all != 0.f ? o[e][k] / all : 0.f);
+        }
+    if (lane == 0 && p.lse != nullptr)
+        p.lse[(int64_t)token * p.kv_heads * (int)p.group.d + head] = all == 0.f ? -INFINITY : (most + log2f(all)) * kLn2;
 }
 
 template <typename T>

@@ -11,9 +11,9 @@
 //     warp, which alone knows the schedule, runs ahead and hands the others a description of each piece of work through a ring of two.
 //   * K and V come in boxes of 8 to 128 rows, a lane of the copying warp to a box, which also looks up its page.
 //   * Q's rows are (token, head) pairs in any layout: every softmax thread fetches its own.
-//   * Keys of a step that the piece does not have (behind its last, in front of the window, of a page that is not there) are masked,
-//     and their rows of V set to zero by the copying warp before the multiplication hears of them: what the cache holds there may be NaN.
-//     (Rows that come out not finite for a key that only others see: row_again.)
+//   * Keys that a row does not see are masked in S.  Rows of V behind the request's last token, or of a page that is not there, are
+//     set to zero by the copying warp before the multiplication hears of them: what the cache holds there may be NaN as a rule.  Where a
+//     token's own V is not finite, rows that do not see it come out not finite too, are noticed and computed again (row_again).
 #include <cuda.h>
 
 #include <type_traits>
@@ -171,12 +171,12 @@ paged_chunk_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Pr
             x.request = w.b;
             x.whole = w.whole();
             x.part = w.part();
-            const int head = w.head;
+            const int head = w.head, limit = t.u0 + t.count;   // keys of the class
             const int32_t* table = p.table + w.b * p.table_stride;
             hand_over(x);
             auto look_up = [&](int j) -> int {                 // page of the lane's box, or -1
                 const int n = x.first + j * kKeys + lane * box;
-                if (j >= x.steps || lane >= kKeys / box || n >= x.hi || n + box <= x.lo) return -1;
+                if (j >= x.steps || lane >= kKeys / box || n >= limit) return -1;
                 if (t.residue + (int64_t)n * s >= p.table_rows) return -1;
                 const int page = __ldg(table + class_page.div(n));
                 return page >= 0 && page < p.pages ? page : -1;
@@ -185,14 +185,14 @@ paged_chunk_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Pr
             for (int j = 0; j < x.steps && ok; ++j, ++n_step) {
                 const int n0 = x.first + j * kKeys, n = n0 + lane * box, slot = n_step % kSlots;
                 const uint32_t turn = ((n_step / kSlots) & 1u) ^ 1u;
-                const int row = n - class_page.div(max(n, 0)) * (int)class_page.d;
+                const int row = n - class_page.div(n) * (int)class_page.d;
                 const uint32_t boxes = __ballot_sync(0xffffffffu, entry >= 0), bytes = __popc(boxes) * box * D * 2;
                 // this lane's four keys of every 128: there?
                 uint32_t there[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int key = i * 32 + lane;
-                    there[i] = __ballot_sync(0xffffffffu, ((boxes >> (key / box)) & 1u) && n0 + key >= x.lo && n0 + key < x.hi);
+                    there[i] = __ballot_sync(0xffffffffu, ((boxes >> (key / box)) & 1u) && n0 + key < limit);
                 }
                 const bool edge = (there[0] & there[1] & there[2] & there[3]) != 0xffffffffu;
                 if (n_step >= kSlots) ok = wait_all(&ctrl->k_free[slot], turn, kErrKFree);
