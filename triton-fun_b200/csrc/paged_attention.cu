@@ -4,6 +4,7 @@
 //     x_j = c tanh(scale q.k_j / c) or scale q.k_j;   s_j = x_j - slope_h (i - j);   o = sum_j e^(s_j - m) v_j / sum_j e^(s_j - m)
 // with m the running maximum; scores, sums and outputs are held in fp32, in powers of two.  How the work is divided: paged_schedule.cuh.
 #include <initializer_list>
+#include <type_traits>
 
 #include "paged_rows.cuh"
 
@@ -18,29 +19,30 @@ __device__ __forceinline__ float score_of(const Problem& p, float dot) {
 // Any type, d up to 256, any strides and alignment: FP32 FMA.  It is what fp32 runs on, and 16-bit operands that the tensor-core
 // kernels cannot fetch.
 //
-// A tile is 8 rows.  kLanes lanes (16 for d <= 64, else the warp) hold a key: each has kCols of its columns and of the 8 rows' q and o.  The
-// 8 dot products are added up over the lanes by halving: 4 + 2 + 1 exchanges leave every lane with one row's sum over some lanes, one
-// or two more complete it (8 to 9 shuffles for 8 sums; one by one they would be 32 to 40).  Four keys are in flight per stream; a
-// block's 4 warps are 4 or 8 streams that share a tile's keys and are joined at its end.
+// A tile is R rows: 8, or 4 or 2 where no request can have more.  kLanes lanes (16 for d <= 64, else the warp) hold a key: each has kCols of
+// its columns and of the rows' q and o.  The R dot products are added up over the lanes by halving: with 8 rows 4 + 2 + 1 exchanges leave
+// every lane with one row's sum over some lanes, one or two more complete it (8 to 9 shuffles for 8 sums; one by one they would be 32 to 40).
+// Issue slots bound it: a key is 22 cycles of HBM (d64), or 89 issue slots, and takes some 54 with 8 rows.  A block's 4 warps are 4 or 8 streams that
+// share a tile's keys and are joined at its end; K and V of a stream's next four keys are on their way while four are worked on.
 // -------------------------------------------------------------------------------------------------
-constexpr int kRowsAny = 8, kKeysAny = 32, kThreadsAny = 128, kBatchAny = 4, kFixedAny = 3;
+constexpr int kKeysAny = 32, kThreadsAny = 128, kPerSmAny = 3, kFixedAny = 3, kSplitAny = 1;
 
-template <int kLanes> __device__ __forceinline__ float reduce_rows(const float (&v)[kRowsAny], int lane) {
-    float w[4], x[2], y;
-    const bool a = lane & (kLanes / 2), b = lane & (kLanes / 4), c = lane & (kLanes / 8);
+template <int kLanes, int R> __device__ __forceinline__ float reduce_rows(float (&v)[R], int lane) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = (a ? v[i + 4] : v[i]) + __shfl_xor_sync(0xffffffffu, a ? v[i] : v[i + 4], kLanes / 2);
+    for (int h = R / 2, o = kLanes / 2; h > 0; h >>= 1, o >>= 1) {
+        const bool upper = lane & o;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) x[i] = (b ? w[i + 2] : w[i]) + __shfl_xor_sync(0xffffffffu, b ? w[i] : w[i + 2], kLanes / 4);
-    y = (c ? x[1] : x[0]) + __shfl_xor_sync(0xffffffffu, c ? x[0] : x[1], kLanes / 8);
+        for (int i = 0; i < R / 2; ++i)
+            if (i < h) v[i] = (upper ? v[i + h] : v[i]) + __shfl_xor_sync(0xffffffffu, upper ? v[i] : v[i + h], o);
+    }
+    float y = v[0];
 #pragma unroll
-    for (int o = kLanes / 16; o > 0; o >>= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
+    for (int o = kLanes / (2 * R); o > 0; o >>= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
     return y;
 }
-// the lane of a group that holds row r's sum
-template <int kLanes> __device__ __forceinline__ int lane_of_row(int r) {
-    return (r & 4 ? kLanes / 2 : 0) + (r & 2 ? kLanes / 4 : 0) + (r & 1 ? kLanes / 8 : 0);
-}
+// the first lane of a group that holds row r's sum (kLanes / R of them do), and a lane's row
+template <int kLanes, int R> __device__ __forceinline__ constexpr int lane_of_row(int r) { return r * (kLanes / R); }
+template <int kLanes, int R> __device__ __forceinline__ constexpr int row_of_lane(int lane) { return lane / (kLanes / R); }
 
 template <typename T, int kCols>
 __device__ __forceinline__ void load_cols(const T* row, int col0, int d, bool wide, float (&x)[kCols]) {
@@ -66,36 +68,44 @@ __device__ __forceinline__ void load_cols(const T* row, int col0, int d, bool wi
     }
 }
 
-template <typename T, int kLanes, int kCols>
-__global__ void __launch_bounds__(kThreadsAny) paged_rows_kernel(const Problem p, const bool wide) {
-    constexpr int kStreams = kThreadsAny / kLanes, kD = kLanes * kCols;
-    using Part = Walk<kRowsAny, kKeysAny, kThreadsAny, kFixedAny>;
+template <typename T, int kLanes, int kCols, int R>
+__global__ void __launch_bounds__(kThreadsAny, kCols == 4 ? kPerSmAny : 2) paged_rows_kernel(const Problem p, const bool wide) {
+    constexpr int kStreams = kThreadsAny / kLanes, kD = kLanes * kCols, kBatch = kCols == 4 ? 4 : 2;       // keys of a stream's round
+    using Part = Walk<R, kKeysAny, kThreadsAny, kFixedAny, kSplitAny>;
     __shared__ union Shared {
         WalkShared<kThreadsAny> walk;
-        struct { float m[kStreams][kRowsAny], l[kStreams][kRowsAny], o[kStreams][kRowsAny][kD]; } join;
+        struct { float m[kStreams][R], l[kStreams][R], o[kStreams][R][kD]; } join;
     } sh;
     const int lane = threadIdx.x & 31, in_group = lane & (kLanes - 1), stream = threadIdx.x / kLanes;
     const int col0 = in_group * kCols;
     depend_wait();
     depend_release();
-    Part w;
-    const bool any = w.start(p, sh.walk);
-    if (threadIdx.x == 0) p.begins[blockIdx.x] = any && !w.begins() ? w.tile_begin : -1;
-    if (!any) return;
+    __shared__ Part w;                                         // (in shared memory, since registers are short)
+    __shared__ bool more;
+    {
+        Part mine;
+        const bool any = mine.start(p, sh.walk);
+        if (threadIdx.x == 0) {
+            p.begins[blockIdx.x] = any && !mine.begins() ? mine.tile_begin : -1;
+            w = mine;
+        }
+        if (!any) return;
+        __syncthreads();
+    }
     const int g = (int)p.group.d, s = (int)p.stride.d;
     do {
         const TileRows t = TileRows::of(p, w);
         const int32_t* table = p.table + w.b * p.table_stride;
         // this lane's row, and all rows' q
-        const int own = ((in_group & (kLanes / 2)) ? 4 : 0) + ((in_group & (kLanes / 4)) ? 2 : 0) + ((in_group & (kLanes / 8)) ? 1 : 0);
+        const int own = row_of_lane<kLanes, R>(in_group);
         auto token_of = [&](int r) {                       // index of the row's token in its class, or -1
-            const int m = p.group.div(w.tile * kRowsAny + r);
+            const int m = p.group.div(w.tile * R + r);
             return m < t.count ? m : -1;
         };
-        auto head_of = [&](int r, int m) { return w.head * g + w.tile * kRowsAny + r - m * g; };
-        float q[kRowsAny][kCols], o[kRowsAny][kCols];
+        auto head_of = [&](int r, int m) { return w.head * g + w.tile * R + r - m * g; };
+        float q[R][kCols], o[R][kCols];
 #pragma unroll
-        for (int r = 0; r < kRowsAny; ++r) {
+        for (int r = 0; r < R; ++r) {
             const int m = token_of(r);
 #pragma unroll
             for (int i = 0; i < kCols; ++i) q[r][i] = o[r][i] = 0.f;
@@ -106,42 +116,65 @@ __global__ void __launch_bounds__(kThreadsAny) paged_rows_kernel(const Problem p
         const int own_m = token_of(own);
         const int own_u = own_m >= 0 ? t.u0 + own_m : INT32_MIN / 2;                   // sees keys (own_u - taps, own_u]
         const float slope = own_m >= 0 && p.slopes != nullptr ? p.slopes[head_of(own, own_m)] * kLog2e * (float)s : 0.f;
-        const int m_first = token_of(0), m_last = min(p.group.div(w.tile * kRowsAny + kRowsAny - 1), t.count - 1);
+        const int m_first = token_of(0), m_last = min(p.group.div(w.tile * R + R - 1), t.count - 1);
         const int lo = max(m_first < 0 ? 0 : t.u0 + m_first - p.taps + 1, w.first_step() * kKeysAny);
         const int hi = m_first < 0 ? 0 : min(t.u0 + m_last + 1, w.last_step() * kKeysAny);
         float top = -INFINITY, sum = 0.f;                   // of the lane's row, over the stream's keys
         const T* kb = static_cast<const T*>(p.k) + w.head * p.k_head;
         const T* vb = static_cast<const T*>(p.v) + w.head * p.v_head;
-        for (int n0 = max(lo, 0); n0 < hi; n0 += kStreams * kBatchAny) {               // (the same for all threads: shuffles inside)
-            const int n = n0 + stream * kBatchAny;
-            float x[kBatchAny];
-            int64_t at[kBatchAny];
-            bool edge = false;
-            {
-                float k[kBatchAny][kCols];
+        // A round is kBatch keys for each stream.  Places are looked up for several rounds at once, a key to a lane, and K and V of a round are
+        // requested before the round in front of it is worked on.
+        constexpr int kOfWarp = kBatch * (32 / kLanes), kRounds = 32 / kOfWarp;        // keys of a warp in a round; rounds of a lookup
+        const int begin = max(lo, 0), rounds = hi > begin ? (hi - begin + kStreams * kBatch - 1) / (kStreams * kBatch) : 0;
+        auto key_of = [&](int round, int i) { return begin + (round * kStreams + (int)(threadIdx.x >> 5) * (32 / kLanes)) * kBatch + i; };   // i-th of the warp's
+        int next_page, next_row, page, row;
+        auto look_up = [&](int round) {
+            const int n = key_of(round + lane / kOfWarp, lane % kOfWarp);
+            const int64_t j = t.residue + (int64_t)n * s;
+            next_page = -1;
+            next_row = 0;
+            if (n < hi && j < p.table_rows) {
+                const int at = p.page_div.div((int)j);
+                next_row = (int)j - at * (int)p.page_div.d;
+                next_page = __ldg(table + at);
+                if (next_page < 0 || next_page >= p.pages) next_page = -1;
+            }
+        };
+        float k[2][kBatch][kCols], v[2][kBatch][kCols];
+        uint32_t there[2] = {0, 0};                         // keys of the stream's batch
+        auto request = [&](int round, float (&k)[kBatch][kCols], float (&v)[kBatch][kCols], uint32_t& there) {
+            there = 0;
 #pragma unroll
-                for (int i = 0; i < kBatchAny; ++i) {
-                    at[i] = n + i < hi ? cache_row(p, table, t.residue + (int64_t)(n + i) * s, p.k_page, p.k_row) : -1;
+            for (int i = 0; i < kBatch; ++i) {
+                const int from = (round % kRounds) * kOfWarp + (lane / kLanes) * kBatch + i;
+                const int at_page = __shfl_sync(0xffffffffu, page, from), at_row = __shfl_sync(0xffffffffu, row, from);
 #pragma unroll
-                    for (int c = 0; c < kCols; ++c) k[i][c] = 0.f;
-                    if (at[i] >= 0) load_cols<T, kCols>(kb + at[i], col0, p.d, wide, k[i]);
-                }
-#pragma unroll
-                for (int i = 0; i < kBatchAny; ++i) {
-                    float dot[kRowsAny];
-#pragma unroll
-                    for (int r = 0; r < kRowsAny; ++r) {
-                        dot[r] = 0.f;
-#pragma unroll
-                        for (int c = 0; c < kCols; ++c) dot[r] = fmaf(q[r][c], k[i][c], dot[r]);
-                    }
-                    x[i] = reduce_rows<kLanes>(dot, in_group);
+                for (int c = 0; c < kCols; ++c) k[i][c] = v[i][c] = 0.f;
+                if (at_page >= 0) {
+                    there |= 1u << i;
+                    load_cols<T, kCols>(kb + at_page * p.k_page + at_row * p.k_row, col0, p.d, wide, k[i]);
+                    load_cols<T, kCols>(vb + at_page * p.v_page + at_row * p.v_row, col0, p.d, wide, v[i]);
                 }
             }
-            float most = top;
+        };
+        auto work = [&](int round, const float (&k)[kBatch][kCols], const float (&v)[kBatch][kCols], uint32_t there) {
+            const int n = key_of(round, (lane / kLanes) * kBatch);
+            float x[kBatch], most = top;
+            bool edge = false;
 #pragma unroll
-            for (int i = 0; i < kBatchAny; ++i) {
-                const bool seen = at[i] >= 0 && n + i <= own_u && n + i > own_u - p.taps;
+            for (int i = 0; i < kBatch; ++i) {
+                float dot[R];
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    dot[r] = 0.f;
+#pragma unroll
+                    for (int c = 0; c < kCols; ++c) dot[r] = fmaf(q[r][c], k[i][c], dot[r]);
+                }
+                x[i] = reduce_rows<kLanes, R>(dot, in_group);
+            }
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) {
+                const bool seen = ((there >> i) & 1u) && n + i <= own_u && n + i > own_u - p.taps;
                 x[i] = seen ? score_of(p, x[i]) - slope * (float)(own_u - n - i) : -INFINITY;
                 edge = edge || !seen;
                 most = fmaxf(most, x[i]);
@@ -151,30 +184,22 @@ __global__ void __launch_bounds__(kThreadsAny) paged_rows_kernel(const Problem p
             const bool moved = __any_sync(0xffffffffu, most > top);
             top = most;
 #pragma unroll
-            for (int i = 0; i < kBatchAny; ++i) x[i] = x[i] == -INFINITY ? 0.f : exp2f(x[i] - base);
+            for (int i = 0; i < kBatch; ++i) x[i] = x[i] == -INFINITY ? 0.f : exp2f(x[i] - base);
             if (moved) {
                 sum *= corr;
 #pragma unroll
-                for (int r = 0; r < kRowsAny; ++r) {
-                    const float f = __shfl_sync(0xffffffffu, corr, (lane & ~(kLanes - 1)) | lane_of_row<kLanes>(r));
+                for (int r = 0; r < R; ++r) {
+                    const float f = __shfl_sync(0xffffffffu, corr, (lane & ~(kLanes - 1)) | lane_of_row<kLanes, R>(r));
 #pragma unroll
                     for (int c = 0; c < kCols; ++c) o[r][c] *= f;
                 }
             }
-            float v[kBatchAny][kCols];
 #pragma unroll
-            for (int i = 0; i < kBatchAny; ++i) {
-#pragma unroll
-                for (int c = 0; c < kCols; ++c) v[i][c] = 0.f;
-                if (at[i] >= 0)
-                    load_cols<T, kCols>(vb + cache_row(p, table, t.residue + (int64_t)(n + i) * s, p.v_page, p.v_row), col0, p.d, wide, v[i]);
-            }
-#pragma unroll
-            for (int i = 0; i < kBatchAny; ++i) {
+            for (int i = 0; i < kBatch; ++i) {
                 sum += x[i];
 #pragma unroll
-                for (int r = 0; r < kRowsAny; ++r) {
-                    const float f = __shfl_sync(0xffffffffu, x[i], (lane & ~(kLanes - 1)) | lane_of_row<kLanes>(r));
+                for (int r = 0; r < R; ++r) {
+                    const float f = __shfl_sync(0xffffffffu, x[i], (lane & ~(kLanes - 1)) | lane_of_row<kLanes, R>(r));
                     // a key that a row does not see may hold anything: 0 times infinity would be NaN
                     if (!edge || f != 0.f) {
 #pragma unroll
@@ -182,21 +207,40 @@ __global__ void __launch_bounds__(kThreadsAny) paged_rows_kernel(const Problem p
                     }
                 }
             }
+        };
+        auto advance = [&](int round) {                     // the places of `round`, if a lookup begins there
+            if (round % kRounds == 0) {
+                page = next_page;
+                row = next_row;
+                look_up(round + kRounds);
+            }
+        };
+        look_up(0);
+        advance(0);
+        request(0, k[0], v[0], there[0]);
+        for (int i = 0; i < rounds; i += 2) {               // (the same for all threads: shuffles inside)
+            advance(i + 1);
+            request(i + 1, k[1], v[1], there[1]);
+            work(i, k[0], v[0], there[0]);
+            if (i + 1 >= rounds) break;
+            advance(i + 2);
+            request(i + 2, k[0], v[0], there[0]);
+            work(i + 1, k[1], v[1], there[1]);
         }
         // the streams' parts, joined
         __syncthreads();
-        if ((in_group & (kLanes / 8 - 1)) == 0) {
+        if ((in_group & (kLanes / R - 1)) == 0) {
             sh.join.m[stream][own] = top;
             sh.join.l[stream][own] = sum;
         }
 #pragma unroll
-        for (int r = 0; r < kRowsAny; ++r)
+        for (int r = 0; r < R; ++r)
 #pragma unroll
             for (int c = 0; c < kCols; ++c) sh.join.o[stream][r][col0 + c] = o[r][c];
         __syncthreads();
         const bool whole = w.whole();
         const int64_t part = w.part();
-        for (int i = threadIdx.x; i < kRowsAny * kD; i += kThreadsAny) {
+        for (int i = threadIdx.x; i < R * kD; i += kThreadsAny) {
             const int r = i / kD, c = i - r * kD, m = token_of(r);
             float most = -INFINITY, all = 0.f, y = 0.f;
             for (int j = 0; j < kStreams; ++j) most = fmaxf(most, sh.join.m[j][r]);
@@ -208,8 +252,8 @@ __global__ void __launch_bounds__(kThreadsAny) paged_rows_kernel(const Problem p
             }
             const int token = m >= 0 ? w.r.first + w.cls + m * s : -1, head = m >= 0 ? head_of(r, m) : 0;
             if (!whole) {
-                if (c == 0) p.part_rows[part * kRowsAny + r] = make_float4(most, all, __int_as_float(token), __int_as_float(head));
-                p.part_o[(part * kRowsAny + r) * kD + c] = y;
+                if (c == 0) p.part_rows[part * R + r] = make_float4(most, all, __int_as_float(token), __int_as_float(head));
+                p.part_o[(part * R + r) * kD + c] = y;
             } else if (token >= 0) {
                 if (c < p.d)
                     static_cast<T*>(p.o)[token * p.o_row + head * p.o_head + c] = DT<T>::from_f(all != 0.f ? y / all : 0.f);
@@ -218,26 +262,27 @@ __global__ void __launch_bounds__(kThreadsAny) paged_rows_kernel(const Problem p
             }
         }
         __syncthreads();
-    } while (w.next(p));
+        if (threadIdx.x == 0) more = w.next(p);
+        __syncthreads();
+    } while (more);
 }
 
 // -------------------------------------------------------------------------------------------------
 // Parts of divided tiles -> results.  Block (c, y): the tile that CTA c begins in the middle of, if no CTA before it does too; a warp per
 // row.  It runs behind the kernel that wrote them, as a launch that is already waiting when that ends.
 // -------------------------------------------------------------------------------------------------
-constexpr int kThreadsJoin = 256;
+constexpr int kThreadsJoin = 512;
 
 template <typename T, int kD>
 __global__ void __launch_bounds__(kThreadsJoin) paged_join_kernel(const Problem p, const int ctas, const int rows) {
     constexpr int kEach = (kD + 127) / 128;                // pieces of 4 columns of a lane
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = blockIdx.x + 1;
-    const int r = blockIdx.y * (kThreadsJoin / 32) + warp;
     depend_wait();
     depend_release();
     // One look at the CTA's neighbours: c - 1, c, c + 1, ... by lane
     const int64_t seen = c - 1 + lane < ctas ? p.begins[c - 1 + lane] : -1;
     const int64_t id = __shfl_sync(0xffffffffu, seen, 1);
-    if (id < 0 || __shfl_sync(0xffffffffu, seen, 0) == id || r >= rows) return;
+    if (id < 0 || __shfl_sync(0xffffffffu, seen, 0) == id) return;
     const unsigned same = __ballot_sync(0xffffffffu, seen == id) >> 1;
     int n = 1 + __ffs(~same) - 1;                          // parts
     for (int j = c + 31; n == 32 + j - c - 31 && j < ctas; j += 32) {      // (more than 31 CTAs begin in the middle of the tile)
@@ -245,76 +290,78 @@ __global__ void __launch_bounds__(kThreadsJoin) paged_join_kernel(const Problem 
         n += more == 0xffffffffu ? 32 : __ffs(~more) - 1;
         if (more != 0xffffffffu) break;
     }
-    auto part = [&](int i) { return (int64_t)(i == 0 ? 2 * (c - 1) + 1 : 2 * (c - 1 + i)) * rows + r; };
-    // The first parts' columns are requested together with the maxima and sums
-    constexpr int kAhead = 4;
-    float4 x[kAhead][kEach];
+    for (int r = blockIdx.y * (kThreadsJoin / 32) + warp; r < rows; r += gridDim.y * (kThreadsJoin / 32)) {
+        auto part = [&](int i) { return (int64_t)(i == 0 ? 2 * (c - 1) + 1 : 2 * (c - 1 + i)) * rows + r; };
+        // The first parts' columns are requested together with the maxima and sums
+        constexpr int kAhead = 4;
+        float4 x[kAhead][kEach];
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i)
-#pragma unroll
-        for (int e = 0; e < kEach; ++e) {
-            const int col = e * 128 + lane * 4;
-            x[i][e] = i < n && col < kD ? *reinterpret_cast<const float4*>(p.part_o + part(i) * kD + col) : make_float4(0.f, 0.f, 0.f, 0.f);
-        }
-    float4 mine = lane < n ? p.part_rows[part(lane)] : make_float4(-INFINITY, 0.f, 0.f, 0.f);
-    const int token = __float_as_int(__shfl_sync(0xffffffffu, mine.z, 0)), head = __float_as_int(__shfl_sync(0xffffffffu, mine.w, 0));
-    if (token < 0) return;
-    float most = mine.x;
-    for (int i = 32 + lane; i < n; i += 32) most = fmaxf(most, p.part_rows[part(i)].x);
-    most = warp_max(most);
-    const float base = most == -INFINITY ? 0.f : most;
-    float all = 0.f, o[kEach][4];
-#pragma unroll
-    for (int e = 0; e < kEach; ++e)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) o[e][k] = 0.f;
-    auto add = [&](float f, const float4& y, int e) {
-        o[e][0] = fmaf(f, y.x, o[e][0]);
-        o[e][1] = fmaf(f, y.y, o[e][1]);
-        o[e][2] = fmaf(f, y.z, o[e][2]);
-        o[e][3] = fmaf(f, y.w, o[e][3]);
-    };
-    for (int i0 = 0; i0 < n; i0 += 32) {
-        if (i0 > 0) mine = i0 + lane < n ? p.part_rows[part(i0 + lane)] : make_float4(-INFINITY, 0.f, 0.f, 0.f);
-        const float f = exp2f(mine.x - base);
-        all = fmaf(f, mine.y, all);
-        const int here = min(32, n - i0);
-        int i = 0;
-        if (i0 == 0) {
-#pragma unroll
-            for (; i < kAhead; ++i) {
-                const float fi = __shfl_sync(0xffffffffu, f, i);
-                if (i < n)
-#pragma unroll
-                    for (int e = 0; e < kEach; ++e) add(fi, x[i][e], e);
-            }
-        }
-#pragma unroll 8
-        for (; i < here; ++i) {
-            const float fi = __shfl_sync(0xffffffffu, f, i);
+        for (int i = 0; i < kAhead; ++i)
 #pragma unroll
             for (int e = 0; e < kEach; ++e) {
                 const int col = e * 128 + lane * 4;
-                if (col < kD) add(fi, *reinterpret_cast<const float4*>(p.part_o + part(i0 + i) * kD + col), e);
+                x[i][e] = i < n && col < kD ? *reinterpret_cast<const float4*>(p.part_o + part(i) * kD + col) : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+        float4 mine = lane < n ? p.part_rows[part(lane)] : make_float4(-INFINITY, 0.f, 0.f, 0.f);
+        const int token = __float_as_int(__shfl_sync(0xffffffffu, mine.z, 0)), head = __float_as_int(__shfl_sync(0xffffffffu, mine.w, 0));
+        if (token < 0) continue;
+        float most = mine.x;
+        for (int i = 32 + lane; i < n; i += 32) most = fmaxf(most, p.part_rows[part(i)].x);
+        most = warp_max(most);
+        const float base = most == -INFINITY ? 0.f : most;
+        float all = 0.f, o[kEach][4];
+#pragma unroll
+        for (int e = 0; e < kEach; ++e)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) o[e][k] = 0.f;
+        auto add = [&](float f, const float4& y, int e) {
+            o[e][0] = fmaf(f, y.x, o[e][0]);
+            o[e][1] = fmaf(f, y.y, o[e][1]);
+            o[e][2] = fmaf(f, y.z, o[e][2]);
+            o[e][3] = fmaf(f, y.w, o[e][3]);
+        };
+        for (int i0 = 0; i0 < n; i0 += 32) {
+            if (i0 > 0) mine = i0 + lane < n ? p.part_rows[part(i0 + lane)] : make_float4(-INFINITY, 0.f, 0.f, 0.f);
+            const float f = exp2f(mine.x - base);
+            all = fmaf(f, mine.y, all);
+            const int here = min(32, n - i0);
+            int i = 0;
+            if (i0 == 0) {
+#pragma unroll
+                for (; i < kAhead; ++i) {
+                    const float fi = __shfl_sync(0xffffffffu, f, i);
+                    if (i < n)
+#pragma unroll
+                        for (int e = 0; e < kEach; ++e) add(fi, x[i][e], e);
+                }
+            }
+#pragma unroll 8
+            for (; i < here; ++i) {
+                const float fi = __shfl_sync(0xffffffffu, f, i);
+#pragma unroll
+                for (int e = 0; e < kEach; ++e) {
+                    const int col = e * 128 + lane * 4;
+                    if (col < kD) add(fi, *reinterpret_cast<const float4*>(p.part_o + part(i0 + i) * kD + col), e);
+                }
             }
         }
+        all = warp_sum(all);
+        T* out = static_cast<T*>(p.o) + token * p.o_row + head * p.o_head;
+#pragma unroll
+        for (int e = 0; e < kEach; ++e)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int col = e * 128 + lane * 4 + k;
+                if (col < p.d) out[col] = DT<T>::from_f(all != 0.f ? o[e][k] / all : 0.f);
+            }
+        if (lane == 0 && p.lse != nullptr)
+            p.lse[(int64_t)token * p.kv_heads * (int)p.group.d + head] = all == 0.f ? -INFINITY : (most + log2f(all)) * kLn2;
     }
-    all = warp_sum(all);
-    T* out = static_cast<T*>(p.o) + token * p.o_row + head * p.o_head;
-#pragma unroll
-    for (int e = 0; e < kEach; ++e)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const int col = e * 128 + lane * 4 + k;
-            if (col < p.d) out[col] = DT<T>::from_f(all != 0.f ? o[e][k] / all : 0.f);
-        }
-    if (lane == 0 && p.lse != nullptr)
-        p.lse[(int64_t)token * p.kv_heads * (int)p.group.d + head] = all == 0.f ? -INFINITY : (most + log2f(all)) * kLn2;
 }
 
 template <typename T>
 static int32_t join_as(const Problem& p, int ctas, int rows, int d_pad, cudaStream_t st) {
-    const dim3 grid((unsigned)(ctas - 1), (unsigned)((rows + kThreadsJoin / 32 - 1) / (kThreadsJoin / 32)));
+    const dim3 grid((unsigned)(ctas - 1), (unsigned)(rows > 16 ? 4 : 1));
     auto kern = d_pad == 64 ? paged_join_kernel<T, 64> : d_pad == 128 ? paged_join_kernel<T, 128> : paged_join_kernel<T, 256>;
     return launch_kernel(kern, grid, dim3(kThreadsJoin), 0, st, p, ctas, rows);
 }
@@ -337,8 +384,18 @@ static int sm_count() {
     return n;
 }
 
-constexpr int kPerSmAny = 3;
 static int d_pad_any(int64_t d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
+
+// most rows that a request's class can have
+static int64_t chunk_rows(const splat_paged_args& a) {
+    const int64_t n = a.max_q_len < a.tokens ? a.max_q_len : a.tokens;
+    return (n / a.stride + (n % a.stride != 0)) * (a.heads / a.kv_heads);
+}
+// Rows of a tile.  us, fp32 B32 kv 4096 H32/8 d128, one token (4 rows): 8 331, 4 see DESIGN; more than the rows there are cost what rows do
+static int rows_any(const splat_paged_args& a) {
+    const int64_t most = chunk_rows(a);
+    return most <= 2 ? 2 : most <= 4 ? 4 : 8;
+}
 
 template <typename T>
 static int32_t launch_any(const splat_paged_args& a, Problem p, int ctas, cudaStream_t st) {
@@ -351,10 +408,18 @@ static int32_t launch_any(const splat_paged_args& a, Problem p, int ctas, cudaSt
     };
     const bool wide = a.d % piece == 0 && fits(a.q, {a.q_row, a.q_head}) && fits(a.k_cache, {a.k_page, a.k_head, a.k_row}) &&
                       fits(a.v_cache, {a.v_page, a.v_head, a.v_row});
-    Layout(ctas, kRowsAny, d_pad_any(a.d)).place(p, a.workspace);
-    auto kern = a.d <= 64 ? paged_rows_kernel<T, 16, kCols> : a.d <= 128 ? paged_rows_kernel<T, 32, kCols> : paged_rows_kernel<T, 32, 2 * kCols>;
+    const int rows = rows_any(a), d_pad = d_pad_any(a.d);
+    Layout(ctas, rows, d_pad).place(p, a.workspace);
+    auto of = [&](auto lanes, auto cols) {
+        constexpr int kLanes = decltype(lanes)::value, kC = decltype(cols)::value;
+        return rows == 8 ? paged_rows_kernel<T, kLanes, kC, 8> : rows == 4 ? paged_rows_kernel<T, kLanes, kC, 4> : paged_rows_kernel<T, kLanes, kC, 2>;
+    };
+    using std::integral_constant;
+    auto kern = d_pad == 64    ? of(integral_constant<int, 16>(), integral_constant<int, kCols>())
+                : d_pad == 128 ? of(integral_constant<int, 32>(), integral_constant<int, kCols>())
+                               : of(integral_constant<int, 32>(), integral_constant<int, 2 * kCols>());
     const int32_t rc = launch_kernel(kern, dim3((unsigned)ctas), dim3(kThreadsAny), 0, st, p, wide);
-    return rc != SPLAT_OK ? rc : join_parts(p, ctas, kRowsAny, d_pad_any(a.d), a.dtype, st);
+    return rc != SPLAT_OK ? rc : join_parts(p, ctas, rows, d_pad, a.dtype, st);
 }
 
 static int32_t check_args(const splat_paged_args& a) {
@@ -410,12 +475,6 @@ int32_t attend_decode(const splat_paged_args& a, Problem p, int sms, void* works
 int chunk_ctas(int sms);
 int32_t attend_chunk(const splat_paged_args& a, Problem p, int sms, void* workspace, cudaStream_t st);
 constexpr int kFewRows = 16;           // rows of a request's class up to which paged_decode.cu takes it
-// most rows that a request's class can have
-static int64_t chunk_rows(const splat_paged_args& a) {
-    const int64_t n = a.max_q_len < a.tokens ? a.max_q_len : a.tokens;
-    return (n / a.stride + (n % a.stride != 0)) * (a.heads / a.kv_heads);
-}
-
 }  // namespace paged
 }  // namespace splat
 
@@ -427,7 +486,7 @@ extern "C" int64_t splat_paged_attention_workspace(const splat_paged_args* a) {
         const int64_t few = Layout(decode_ctas(sms), 16, d_pad_any(a->d)).bytes, many = Layout(chunk_ctas(sms), 128, d_pad_any(a->d)).bytes;
         return chunk_rows(*a) > kFewRows && many > few ? many : few;
     }
-    return Layout(sms * kPerSmAny, kRowsAny, d_pad_any(a->d)).bytes;
+    return Layout(sms * kPerSmAny, rows_any(*a), d_pad_any(a->d)).bytes;
 }
 
 extern "C" int32_t splat_paged_attention(const splat_paged_args* args, void* stream) {
@@ -469,7 +528,9 @@ extern "C" int32_t splat_paged_attention(const splat_paged_args* args, void* str
         // Requests of few rows and of many, one after the other where there may be both; they share the workspace, which is why the
         // second waits for the joining of the first
         if (chunk_rows(a) > kFewRows) {
-            const bool alike = a.tokens == a.requests * a.max_q_len;           // as a rule: all of them bring as many
+            // One kernel for all of them where, as a rule, all bring as many, or where those of few rows are so few that a launch of their own
+            // costs more than tiles that are mostly empty (8 requests, 2 of them with chunks, 8 heads: 69 us with two launches, 46 with one)
+            const bool alike = a.tokens == a.requests * a.max_q_len || a.requests * a.kv_heads <= chunk_ctas(sms) / 2;
             p.rows_from = alike ? 0 : kFewRows + 1;
             const int32_t rc = attend_chunk(a, p, sms, a.workspace, st);
             if (rc != SPLAT_ERR_UNSUPPORTED_SHAPE) {

@@ -33,6 +33,7 @@ using sm::pack2;
 
 constexpr int kRows = 128, kKeys = 128, kThreads = 192, kTmaWarp = 4, kMmaWarp = 5;
 constexpr int kFixed = 3;                       // what a tile costs beside its steps, in steps
+constexpr int kSplit = 6;                       // what dividing one costs
 constexpr int kTmemCols = 256, kPerSm = 2;
 constexpr float kLazy = 8.f;                    // log2: the maximum is raised when it has grown by more
 enum : int { kErrPiece = 91, kErrPieceFree, kErrQ, kErrKFull, kErrKFree, kErrVFull, kErrVFree, kErrVLanded, kErrS, kErrSFree, kErrP, kErrPv, kErrO };
@@ -87,7 +88,7 @@ template <typename T, int D, bool kMod>
 __global__ void __launch_bounds__(kThreads, kPerSm)
 paged_chunk_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Problem p, const int box, const FastDiv class_page, const bool q_wide) {
     using S = Shape<D>;
-    using Part = Walk<kRows, kKeys, kThreads, kFixed>;
+    using Part = Walk<kRows, kKeys, kThreads, kFixed, kSplit>;
     constexpr int kSlots = S::kSlots;
     constexpr bool kOwnP = D == 64;                            // P has tensor-memory columns of its own
     constexpr uint32_t kPCol = kOwnP ? kKeys + D : 0;

@@ -34,7 +34,8 @@ using sm::ex2;
 using sm::pack2;
 
 constexpr int kWarps = 4, kThreads = 160, kCopyWarp = 4, kRows = 16, kSlots = 8;
-constexpr int kFixed = 3;            // what a tile costs beside its steps, in steps
+constexpr int kFixed = 2;            // what a tile costs beside its steps, in steps (us, the two cases: 0 155 / 140, 1 91 / 93, 2 85.6 / 80.3, 4 86.4 / 81.7)
+constexpr int kSplit = 1;            // what dividing one costs
 constexpr float kLazy = 8.f;         // log2: the maximum is raised when it has grown by more
 
 // codes of the status word
@@ -116,7 +117,7 @@ template <typename T, int D, bool kTma>
 __global__ void __launch_bounds__(kThreads, Shape<D>::kPerSm)
 paged_decode_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Problem p, const int box, const FastDiv class_page, const bool q_wide) {
     using S = Shape<D>;
-    using Part = Walk<kRows, S::kKeys, kThreads, kFixed>;
+    using Part = Walk<kRows, S::kKeys, kThreads, kFixed, kSplit>;
     constexpr int kChunk = S::kChunk;
     extern __shared__ uint8_t smem_raw[];
     __shared__ WalkShared<kThreads> walk;

@@ -17,6 +17,9 @@
 // that a CTA that came by the short requests of a ragged batch took three times as long as the others: 64 decoding requests of 1 to
 // 16384 tokens (log-uniform), 32 / 8 heads, d128 bf16 249 us without.
 //
+// Dividing a tile has a price too (a second fetch of its rows, parts out and in again), kSplit steps; where whole tiles come out no
+// worse than that (as a rule where there is less than one for each CTA), they are handed out whole.
+//
 // Steps are counted for a class of a request's longest kind, so that all of its classes and heads have the same tiles; where the count
 // is one too high a CTA has a step without keys.
 #pragma once
@@ -91,11 +94,13 @@ __device__ __forceinline__ int2 steps_of(const Problem& p, const Request& r, int
     return make_int2(x, max(x + 1, (hi + kKeys - 1) / kKeys));
 }
 template <int R, int kKeys, int kFixed>
-__device__ __forceinline__ int64_t cost_of_class(const Problem& p, const Request& r) {
+__device__ __forceinline__ int64_t cost_of_class(const Problem& p, const Request& r, int& most) {
     int64_t sum = 0;
     for (int t = 0; t < r.tiles; ++t) {
         const int2 s = steps_of<R, kKeys>(p, r, t);
-        sum += s.y - s.x + kFixed;
+        const int cost = s.y - s.x + kFixed;
+        sum += cost;
+        most = max(most, cost);
     }
     return sum;
 }
@@ -104,17 +109,19 @@ __device__ __forceinline__ int64_t divide(int64_t a, int64_t b) {
 }
 
 template <int kThreads> struct WalkShared {
-    int64_t before[kThreads + 1];      // cost in front of a thread's requests
-    int64_t warp_sums[kThreads / 32];
+    int64_t before[kThreads + 1];      // in front of a thread's requests
+    int64_t warp_cost[kThreads / 32], warp_tiles[kThreads / 32];
+    int warp_most[kThreads / 32];
 };
 
 // A CTA's walk over its share.  All threads of the block, the same in each.
-template <int R, int kKeys, int kThreads, int kFixed>
+template <int R, int kKeys, int kThreads, int kFixed, int kSplit>
 struct Walk {
-    int64_t end;                       // of the share, in steps and fixed costs of all tiles
+    int64_t end;                       // of the share, in steps and fixed costs of all tiles; or in tiles, which count 1 then
     int64_t tile_begin;                // of the tile
     int64_t at;                        // where the share begins in it: tile_begin, or behind the fixed cost
     int b, head, cls, tile;
+    bool by_tile;                      // tiles are handed out whole
     Request r;
     int2 steps;                        // of the tile
 
@@ -122,26 +129,41 @@ struct Walk {
     __device__ bool start(const Problem& p, WalkShared<kThreads>& sh) {
         const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
         const int each = (p.requests + kThreads - 1) / kThreads;
-        int64_t mine = 0;
+        int64_t cost_mine = 0, tiles_mine = 0;
+        int most = 0;
         for (int i = 0; i < each; ++i) {
             const int q = threadIdx.x * each + i;
             if (q >= p.requests) break;
             const Request x = request_of<R>(p, q);
-            mine += cost_of_class<R, kKeys, kFixed>(p, x) * x.classes * p.kv_heads;
+            cost_mine += cost_of_class<R, kKeys, kFixed>(p, x, most) * x.classes * p.kv_heads;
+            tiles_mine += (int64_t)x.tiles * x.classes * p.kv_heads;
         }
-        int64_t x = mine;
+        int64_t cost_sum = cost_mine, tiles_sum = tiles_mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
-            if (lane >= o) x += y;
+            const int64_t y = __shfl_up_sync(0xffffffffu, cost_sum, o), z = __shfl_up_sync(0xffffffffu, tiles_sum, o);
+            if (lane >= o) { cost_sum += y; tiles_sum += z; }
         }
-        if (lane == 31) sh.warp_sums[warp] = x;
+        most = warp_max_i(most);
+        if (lane == 31) {
+            sh.warp_cost[warp] = cost_sum;
+            sh.warp_tiles[warp] = tiles_sum;
+            sh.warp_most[warp] = most;
+        }
         __syncthreads();
-        for (int w = 0; w < warp; ++w) x += sh.warp_sums[w];
-        sh.before[threadIdx.x + 1] = x;
+        int64_t cost_all = 0, tiles_all = 0;
+        for (int w = 0; w < kThreads / 32; ++w) {
+            if (w < warp) { cost_sum += sh.warp_cost[w]; tiles_sum += sh.warp_tiles[w]; }
+            cost_all += sh.warp_cost[w];
+            tiles_all += sh.warp_tiles[w];
+            most = max(most, sh.warp_most[w]);
+        }
+        const int64_t cost_share = divide(cost_all + gridDim.x - 1, gridDim.x), tiles_share = divide(tiles_all + gridDim.x - 1, gridDim.x);
+        by_tile = tiles_share * most <= cost_share + kSplit;
+        sh.before[threadIdx.x + 1] = by_tile ? tiles_sum : cost_sum;
         if (threadIdx.x == 0) sh.before[0] = 0;
         __syncthreads();
-        const int64_t all = sh.before[kThreads], share = divide(all + gridDim.x - 1, gridDim.x);
+        const int64_t all = by_tile ? tiles_all : cost_all, share = by_tile ? tiles_share : cost_share;
         at = min((int64_t)blockIdx.x * share, all);
         end = min(at + share, all);
         if (at >= end) return false;
@@ -153,7 +175,7 @@ struct Walk {
         int64_t sum = sh.before[lo], class_cost;
         for (b = lo * each;; ++b) {    // (ends: what is behind `at` is some request's)
             r = request_of<R>(p, b);
-            class_cost = cost_of_class<R, kKeys, kFixed>(p, r);
+            class_cost = by_tile ? r.tiles : cost_of_class<R, kKeys, kFixed>(p, r, most);
             const int64_t w = class_cost * r.classes * p.kv_heads;
             if (at < sum + w) break;
             sum += w;
@@ -164,25 +186,28 @@ struct Walk {
         rest -= head * per_head;
         cls = (int)divide(rest, class_cost);
         rest -= cls * class_cost;
-        for (tile = 0;; ++tile) {
+        tile = by_tile ? (int)rest : 0;
+        if (by_tile) rest = 0;
+        for (;; ++tile) {
             steps = steps_of<R, kKeys>(p, r, tile);
             if (rest < cost()) break;
             rest -= cost();
         }
         tile_begin = at - rest;
-        if (rest <= kFixed) at = tile_begin;             // (the whole of it)
-        return end - tile_begin > kFixed || next(p);
+        if (rest <= fixed()) at = tile_begin;            // (the whole of it)
+        return end - tile_begin > fixed() || next(p);
     }
-    __device__ __forceinline__ int cost() const { return steps.y - steps.x + kFixed; }
+    __device__ __forceinline__ int fixed() const { return by_tile ? 0 : kFixed; }
+    __device__ __forceinline__ int cost() const { return by_tile ? 1 : steps.y - steps.x + kFixed; }
     __device__ __forceinline__ bool begins() const { return at == tile_begin; }
     __device__ __forceinline__ int first_step() const { return begins() ? steps.x : steps.x + (int)(at - tile_begin) - kFixed; }
-    __device__ __forceinline__ int last_step() const { return (int)min((int64_t)steps.y, steps.x + (end - tile_begin - kFixed)); }    // (one behind)
+    __device__ __forceinline__ int last_step() const { return by_tile ? steps.y : (int)min((int64_t)steps.y, steps.x + (end - tile_begin - kFixed)); }    // (one behind)
     __device__ __forceinline__ bool whole() const { return begins() && end - tile_begin >= cost(); }
     __device__ __forceinline__ int part() const { return 2 * blockIdx.x + (begins() ? 1 : 0); }
     // To the next tile; false at the end of the share: a tile of which no step is left in it is the next CTA's.
     __device__ bool next(const Problem& p) {
         at = tile_begin + cost();
-        if (end - at <= kFixed) return false;
+        if (end - at <= fixed()) return false;
         tile_begin = at;
         if (++tile == r.tiles) {
             tile = 0;
@@ -204,7 +229,7 @@ struct TileRows {
     int count;                         // tokens of the class
     int u0;                            // index of its first among the class's keys
     int residue;                       // key n of the class is token residue + n * stride
-    template <int R, int K, int N, int F> __device__ __forceinline__ static TileRows of(const Problem& p, const Walk<R, K, N, F>& w) {
+    template <int R, int K, int N, int F, int S> __device__ __forceinline__ static TileRows of(const Problem& p, const Walk<R, K, N, F, S>& w) {
         TileRows t;
         const int s = (int)p.stride.d, pos = w.r.pos + w.cls;
         t.count = p.stride.div(w.r.n - w.cls + s - 1);
