@@ -268,21 +268,24 @@ __global__ void __launch_bounds__(kThreadsAny, kCols == 4 ? kPerSmAny : 2) paged
 }
 
 // -------------------------------------------------------------------------------------------------
-// Parts of divided tiles -> results.  Block (c, y): the tile that CTA c begins in the middle of, if no CTA before it does too; a warp per
-// row.  It runs behind the kernel that wrote them, as a launch that is already waiting when that ends.
+// Parts of divided tiles -> results.  Block (c, y): the tile that CTA c begins in the middle of, if no CTA before it does too.  It runs behind the
+// kernel that wrote them, as a launch that is already waiting when that ends.  What it costs is round trips to memory, so a row of a small
+// tile, which may have many parts (one request of 8192 tokens: 37), has four warps that take every fourth part each, and the first parts
+// are requested before it is known what they weigh.
 // -------------------------------------------------------------------------------------------------
-constexpr int kThreadsJoin = 512;
+constexpr int kThreadsJoin = 512, kWarpsJoin = kThreadsJoin / 32;
 
-template <typename T, int kD>
+template <typename T, int kD, int kOfRow>                  // kOfRow: warps of a row
 __global__ void __launch_bounds__(kThreadsJoin) paged_join_kernel(const Problem p, const int ctas, const int rows) {
-    constexpr int kEach = (kD + 127) / 128;                // pieces of 4 columns of a lane
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = blockIdx.x + 1;
+    constexpr int kEach = (kD + 127) / 128, kAhead = 4;    // pieces of 4 columns of a lane; parts requested at the start
+    __shared__ float4 shared_o[kOfRow > 1 ? kWarpsJoin : 1][kEach * 32];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = blockIdx.x + 1, which = warp % kOfRow;
     depend_wait();
     depend_release();
     // One look at the CTA's neighbours: c - 1, c, c + 1, ... by lane
     const int64_t seen = c - 1 + lane < ctas ? p.begins[c - 1 + lane] : -1;
     const int64_t id = __shfl_sync(0xffffffffu, seen, 1);
-    if (id < 0 || __shfl_sync(0xffffffffu, seen, 0) == id) return;
+    if (id < 0 || __shfl_sync(0xffffffffu, seen, 0) == id) return;             // (the whole block)
     const unsigned same = __ballot_sync(0xffffffffu, seen == id) >> 1;
     int n = 1 + __ffs(~same) - 1;                          // parts
     for (int j = c + 31; n == 32 + j - c - 31 && j < ctas; j += 32) {      // (more than 31 CTAs begin in the middle of the tile)
@@ -290,86 +293,107 @@ __global__ void __launch_bounds__(kThreadsJoin) paged_join_kernel(const Problem 
         n += more == 0xffffffffu ? 32 : __ffs(~more) - 1;
         if (more != 0xffffffffu) break;
     }
-    for (int r = blockIdx.y * (kThreadsJoin / 32) + warp; r < rows; r += gridDim.y * (kThreadsJoin / 32)) {
+    constexpr int kRowsAtOnce = kWarpsJoin / kOfRow;
+    for (int r0 = blockIdx.y * kRowsAtOnce; r0 < rows; r0 += gridDim.y * kRowsAtOnce) {        // (rows is a multiple, or all rows fit)
+        const int r = r0 + warp / kOfRow;
+        const bool real = r < rows;
         auto part = [&](int i) { return (int64_t)(i == 0 ? 2 * (c - 1) + 1 : 2 * (c - 1 + i)) * rows + r; };
-        // The first parts' columns are requested together with the maxima and sums
-        constexpr int kAhead = 4;
+        auto columns = [&](int i, int e) {
+            const int col = e * 128 + lane * 4;
+            return col < kD ? *reinterpret_cast<const float4*>(p.part_o + part(i) * kD + col) : make_float4(0.f, 0.f, 0.f, 0.f);
+        };
         float4 x[kAhead][kEach];
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i)
+        for (int k = 0; k < kAhead; ++k)
 #pragma unroll
-            for (int e = 0; e < kEach; ++e) {
-                const int col = e * 128 + lane * 4;
-                x[i][e] = i < n && col < kD ? *reinterpret_cast<const float4*>(p.part_o + part(i) * kD + col) : make_float4(0.f, 0.f, 0.f, 0.f);
-            }
-        float4 mine = lane < n ? p.part_rows[part(lane)] : make_float4(-INFINITY, 0.f, 0.f, 0.f);
+            for (int e = 0; e < kEach; ++e)
+                x[k][e] = real && which + k * kOfRow < n ? columns(which + k * kOfRow, e) : make_float4(0.f, 0.f, 0.f, 0.f);
+        float4 mine = real && lane < n ? p.part_rows[part(lane)] : make_float4(-INFINITY, 0.f, __int_as_float(-1), 0.f);
         const int token = __float_as_int(__shfl_sync(0xffffffffu, mine.z, 0)), head = __float_as_int(__shfl_sync(0xffffffffu, mine.w, 0));
-        if (token < 0) continue;
+        float all = 0.f;
+        float4 o[kEach];
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) o[e] = make_float4(0.f, 0.f, 0.f, 0.f);
         float most = mine.x;
-        for (int i = 32 + lane; i < n; i += 32) most = fmaxf(most, p.part_rows[part(i)].x);
-        most = warp_max(most);
-        const float base = most == -INFINITY ? 0.f : most;
-        float all = 0.f, o[kEach][4];
+        if (token >= 0) {
+            for (int i = 32 + lane; i < n; i += 32) most = fmaxf(most, p.part_rows[part(i)].x);
+            most = warp_max(most);
+            const float base = most == -INFINITY ? 0.f : most;
+            auto add = [&](float f, const float4& y, float4& o) {
+                o.x = fmaf(f, y.x, o.x); o.y = fmaf(f, y.y, o.y); o.z = fmaf(f, y.z, o.z); o.w = fmaf(f, y.w, o.w);
+            };
+            for (int i0 = 0; i0 < n; i0 += 32) {
+                if (i0 > 0) mine = i0 + lane < n ? p.part_rows[part(i0 + lane)] : make_float4(-INFINITY, 0.f, 0.f, 0.f);
+                const float f = exp2f(mine.x - base);
+                all = fmaf(f, mine.y, all);
+                const int here = min(32, n - i0);
+                int i = which;
+                if (i0 == 0) {
 #pragma unroll
-        for (int e = 0; e < kEach; ++e)
+                    for (int k = 0; k < kAhead; ++k, i += kOfRow) {
+                        const float fi = __shfl_sync(0xffffffffu, f, i);
+                        if (i < n)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) o[e][k] = 0.f;
-        auto add = [&](float f, const float4& y, int e) {
-            o[e][0] = fmaf(f, y.x, o[e][0]);
-            o[e][1] = fmaf(f, y.y, o[e][1]);
-            o[e][2] = fmaf(f, y.z, o[e][2]);
-            o[e][3] = fmaf(f, y.w, o[e][3]);
-        };
-        for (int i0 = 0; i0 < n; i0 += 32) {
-            if (i0 > 0) mine = i0 + lane < n ? p.part_rows[part(i0 + lane)] : make_float4(-INFINITY, 0.f, 0.f, 0.f);
-            const float f = exp2f(mine.x - base);
-            all = fmaf(f, mine.y, all);
-            const int here = min(32, n - i0);
-            int i = 0;
-            if (i0 == 0) {
-#pragma unroll
-                for (; i < kAhead; ++i) {
-                    const float fi = __shfl_sync(0xffffffffu, f, i);
-                    if (i < n)
-#pragma unroll
-                        for (int e = 0; e < kEach; ++e) add(fi, x[i][e], e);
+                            for (int e = 0; e < kEach; ++e) add(fi, x[k][e], o[e]);
+                    }
                 }
-            }
 #pragma unroll 8
-            for (; i < here; ++i) {
-                const float fi = __shfl_sync(0xffffffffu, f, i);
+                for (; i < here; i += kOfRow) {
+                    const float fi = __shfl_sync(0xffffffffu, f, i);
 #pragma unroll
-                for (int e = 0; e < kEach; ++e) {
-                    const int col = e * 128 + lane * 4;
-                    if (col < kD) add(fi, *reinterpret_cast<const float4*>(p.part_o + part(i0 + i) * kD + col), e);
+                    for (int e = 0; e < kEach; ++e) add(fi, columns(i0 + i, e), o[e]);
                 }
             }
+            all = warp_sum(all);                           // (of all parts, in every warp of the row)
         }
-        all = warp_sum(all);
+        if (kOfRow > 1) {
+#pragma unroll
+            for (int e = 0; e < kEach; ++e) shared_o[warp][e * 32 + lane] = o[e];
+            __syncthreads();
+            if (which == 0)
+#pragma unroll
+                for (int k = 1; k < kOfRow; ++k)
+#pragma unroll
+                    for (int e = 0; e < kEach; ++e) {
+                        const float4 y = shared_o[warp + k][e * 32 + lane];
+                        o[e].x += y.x; o[e].y += y.y; o[e].z += y.z; o[e].w += y.w;
+                    }
+            __syncthreads();
+        }
+        if (token < 0 || which != 0) continue;
         T* out = static_cast<T*>(p.o) + token * p.o_row + head * p.o_head;
 #pragma unroll
-        for (int e = 0; e < kEach; ++e)
+        for (int e = 0; e < kEach; ++e) {
+            const float y[4] = {o[e].x, o[e].y, o[e].z, o[e].w};
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 const int col = e * 128 + lane * 4 + k;
-                if (col < p.d) out[col] = DT<T>::from_f(all != 0.f ? o[e][k] / all : 0.f);
+                if (col < p.d) out[col] = DT<T>::from_f(all != 0.f ? y[k] / all : 0.f);
             }
+        }
         if (lane == 0 && p.lse != nullptr)
             p.lse[(int64_t)token * p.kv_heads * (int)p.group.d + head] = all == 0.f ? -INFINITY : (most + log2f(all)) * kLn2;
     }
 }
 
+template <typename T, int kD>
+static int32_t join_as(const Problem& p, int ctas, int rows, cudaStream_t st) {
+    // Few parts to a tile, as a rule (a tile of each request and head: fewer than four CTAs to each), or many rows: a warp per row.  us, one request of
+    // 8192 tokens, 32 / 8 heads / 32 of 512: one warp 22.2 / 17.4, four 17.6 / 18.9
+    const bool few = (int64_t)p.requests * p.kv_heads * 4 > ctas;
+    if (rows > 16 || few)
+        return launch_kernel(paged_join_kernel<T, kD, 1>, dim3((unsigned)(ctas - 1), rows > 16 ? 4 : 1), dim3(kThreadsJoin), 0, st, p, ctas, rows);
+    return launch_kernel(paged_join_kernel<T, kD, 4>, dim3((unsigned)(ctas - 1), (unsigned)((rows + 3) / 4)), dim3(kThreadsJoin), 0, st, p, ctas, rows);
+}
 template <typename T>
-static int32_t join_as(const Problem& p, int ctas, int rows, int d_pad, cudaStream_t st) {
-    const dim3 grid((unsigned)(ctas - 1), (unsigned)(rows > 16 ? 4 : 1));
-    auto kern = d_pad == 64 ? paged_join_kernel<T, 64> : d_pad == 128 ? paged_join_kernel<T, 128> : paged_join_kernel<T, 256>;
-    return launch_kernel(kern, grid, dim3(kThreadsJoin), 0, st, p, ctas, rows);
+static int32_t join_for(const Problem& p, int ctas, int rows, int d_pad, cudaStream_t st) {
+    return d_pad == 64 ? join_as<T, 64>(p, ctas, rows, st) : d_pad == 128 ? join_as<T, 128>(p, ctas, rows, st) : join_as<T, 256>(p, ctas, rows, st);
 }
 int32_t join_parts(const Problem& p, int ctas, int rows, int d_pad, int32_t dtype, cudaStream_t st) {
     if (ctas < 2) return SPLAT_OK;
-    if (dtype == SPLAT_F32) return join_as<float>(p, ctas, rows, d_pad, st);
-    if (dtype == SPLAT_F16) return join_as<__half>(p, ctas, rows, d_pad, st);
-    return join_as<__nv_bfloat16>(p, ctas, rows, d_pad, st);
+    if (dtype == SPLAT_F32) return join_for<float>(p, ctas, rows, d_pad, st);
+    if (dtype == SPLAT_F16) return join_for<__half>(p, ctas, rows, d_pad, st);
+    return join_for<__nv_bfloat16>(p, ctas, rows, d_pad, st);
 }
 
 // -------------------------------------------------------------------------------------------------
