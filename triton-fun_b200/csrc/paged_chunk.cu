@@ -41,7 +41,7 @@ enum : int { kErrPiece = 91, kErrPieceFree, kErrQ, kErrKFull, kErrKFree, kErrVFu
 struct Maps { CUtensorMap k, v; };
 
 template <int D> struct Shape {
-    static constexpr int kSub = D / 64;
+    static constexpr int kSub = D / 64, kPieces = D / 8;       // boxes of 64 columns; 16-byte pieces of a row
     static constexpr int kSubBytes = kKeys * 128;              // 64 columns of a tile
     static constexpr int kTile = kSub * kSubBytes;             // Q, or a step's K or V
     static constexpr int kSlots = D == 128 ? 1 : 2;            // steps of K, and of V
@@ -175,6 +175,14 @@ paged_chunk_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Pr
             const int head = w.head, limit = t.u0 + t.count;   // keys of the class
             const int32_t* table = p.table + w.b * p.table_stride;
             hand_over(x);
+            if (x.steps > 0) {                                 // its rows of Q, to the L2 cache by the time that they are asked for
+                for (int r = lane; r < kRows; r += 32) {
+                    const int m = rows.token_of(r);
+                    if (m < 0) continue;
+                    const char* q = reinterpret_cast<const char*>(static_cast<const T*>(p.q) + rows.row_of(m) * p.q_row + rows.head_of(r, m) * p.q_head);
+                    for (int i = 0; i < p.d * 2; i += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(q + i));
+                }
+            }
             auto look_up = [&](int j) -> int {                 // page of the lane's box, or -1
                 const int n = x.first + j * kKeys + lane * box;
                 if (j >= x.steps || lane >= kKeys / box || n >= limit) return -1;
@@ -228,12 +236,16 @@ paged_chunk_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Pr
                         break;
                     }
                     ++n_edge;
+#pragma unroll
+                    for (int word = 0; word < 4; ++word) {
+                        if (there[word] == 0xffffffffu) continue;
 #pragma unroll 1
-                    for (int i = 0; i < kKeys / 4; ++i) {      // four rows at a time, eight 16-byte pieces each
-                        const int key = i * 4 + (lane >> 3);
-                        if (((there[key >> 5] >> (key & 31)) & 1u) == 0)
-                            for (int sub = 0; sub < S::kSub; ++sub)
-                                *reinterpret_cast<uint4*>(v_tile + sub * S::kSubBytes + key * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
+                        for (int i = 0; i < 32; i += 4) {      // four rows at a time, eight 16-byte pieces each
+                            const int key = i + (lane >> 3);
+                            if (((there[word] >> key) & 1u) == 0)
+                                for (int sub = 0; sub < S::kSub; ++sub)
+                                    *reinterpret_cast<uint4*>(v_tile + sub * S::kSubBytes + (word * 32 + key) * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
+                        }
                     }
                     fence_proxy_async_smem();
                     __syncwarp();
@@ -345,6 +357,7 @@ paged_chunk_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Pr
         const uint32_t lane_addr = tmem_base + ((uint32_t)(warp * 32) << 16);
         const uint32_t s_addr = lane_addr, o_addr = lane_addr + kKeys, p_addr = lane_addr + kPCol;
         const int t = warp * 32 + lane;                        // row of the tile
+        constexpr int kRowsAtOnce = 32 / S::kPieces;           // of Q and O, in one access of the warp
         const float sc = kMod ? 1.f : p.scale_log2;
         const float2 sc2 = make_float2(sc, sc);
         uint32_t n_piece = 0, n_o = 0, n_step = 0;
@@ -353,54 +366,67 @@ paged_chunk_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Pr
             const uint32_t slot = n_piece & 1;
             ok = wait_all(&ctrl->piece_full[slot], (n_piece >> 1) & 1u, kErrPiece);
             if (!ok) break;
+            // (the piece stays until the end of its epilogue; what the loop does not need is read from it again behind it: registers are short)
             const Piece* const x = &ctrl->piece[slot];
             const int steps = x->steps;
             if (steps < 0) break;
-            const int first = x->first, hi = x->hi, part = x->whole ? -1 : x->part;
-            int token = -1, head = 0, row_lo = 0, row_hi = INT32_MIN / 2;      // keys that the row sees
+            auto token_of_row = [&](int& head) {               // or -1
+                const int m = p.group.div(x->base + t);
+                head = x->head0 + x->base + t - m * (int)p.group.d;
+                return m < x->count ? x->row0 + m * (int)p.stride.d : -1;
+            };
+            int v_lo = 0, v_hi = INT32_MIN / 2, away = 0;      // keys that the row sees, and its own, counted from the step's first
+            float slope = 0.f;
             {
                 const int m = p.group.div(x->base + t);
                 if (m < x->count) {
-                    token = x->row0 + m * (int)p.stride.d;
-                    head = x->head0 + x->base + t - m * (int)p.group.d;
-                    row_hi = x->u0 + m + 1;
-                    row_lo = max(row_hi - p.taps, x->lo);
+                    const int u = x->u0 + m;
+                    away = u - x->first;
+                    v_lo = max(u + 1 - p.taps, x->lo) - x->first;
+                    v_hi = min(u + 1, x->hi) - x->first;
+                    if (kMod && p.slopes != nullptr)
+                        slope = __ldg(p.slopes + x->head0 + x->base + t - m * (int)p.group.d) * kLog2e * (float)(int)p.stride.d;
                 }
             }
-            const float slope = kMod && p.slopes != nullptr && token >= 0 ? __ldg(p.slopes + head) * kLog2e * (float)(int)p.stride.d : 0.f;
-            // (the piece stays until the end of its epilogue, for the rows that are computed again)
             float m_used = -INFINITY, l_sum = 0.f;
             if (steps > 0) {
-                // Q: the last tile's products are complete (o_full), its memory is free
-                const T* src = static_cast<const T*>(p.q) + token * p.q_row + head * p.q_head;
+                // Q: the last tile's products are complete (o_full), its memory is free.  kPieces lanes to a row, 16 bytes each (a lane to a row touches 32
+                // lines with every load)
+                int head;
+                const int token = token_of_row(head);
+                const int64_t from = token >= 0 ? token * p.q_row + head * p.q_head : -1;
+                const int piece = lane % S::kPieces;
+                auto q_at = [&](int row) { return smem + (piece >> 3) * S::kSubBytes + (warp * 32 + row) * 128 + (((piece & 7) ^ (row & 7)) << 4); };
+                if (q_wide) {
+                    uint4 v[32 / kRowsAtOnce];                 // (all requested before the first is stored)
 #pragma unroll
-                for (int sub = 0; sub < S::kSub; ++sub)
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const int col = sub * 64 + i * 8;
-                        uint4 v = make_uint4(0, 0, 0, 0);
-                        if (token >= 0 && col < p.d) {
-                            if (q_wide) {
-                                v = __ldg(reinterpret_cast<const uint4*>(src + col));
-                            } else {
-                                T e[8];
-                                for (int k = 0; k < 8; ++k) e[k] = src[col + k];
-                                v = *reinterpret_cast<const uint4*>(e);
-                            }
-                        }
-                        *reinterpret_cast<uint4*>(smem + sub * S::kSubBytes + t * 128 + ((i ^ (t & 7)) << 4)) = v;
+                    for (int i = 0; i < 32 / kRowsAtOnce; ++i) {
+                        const int64_t at = __shfl_sync(0xffffffffu, from, i * kRowsAtOnce + lane / S::kPieces);
+                        const bool there = at >= 0 && piece * 8 < p.d;
+                        v[i] = make_uint4(0, 0, 0, 0);
+                        if (there) v[i] = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + at + piece * 8));
                     }
+#pragma unroll
+                    for (int i = 0; i < 32 / kRowsAtOnce; ++i) *reinterpret_cast<uint4*>(q_at(i * kRowsAtOnce + lane / S::kPieces)) = v[i];
+                } else {
+#pragma unroll 1
+                    for (int i = 0; i < 32 / kRowsAtOnce; ++i) {
+                        const int64_t at = __shfl_sync(0xffffffffu, from, i * kRowsAtOnce + lane / S::kPieces);
+                        const bool there = at >= 0 && piece * 8 < p.d;
+                        __align__(16) T e[8];
+                        for (int k = 0; k < 8; ++k) e[k] = there ? static_cast<const T*>(p.q)[at + piece * 8 + k] : DT<T>::from_f(0.f);
+                        *reinterpret_cast<uint4*>(q_at(i * kRowsAtOnce + lane / S::kPieces)) = *reinterpret_cast<const uint4*>(e);
+                    }
+                }
                 fence_proxy_async_smem();
                 tc_fence_before_sync();                        // (O of the last tile has been read)
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&ctrl->q_full);
             }
-            for (int k = 0; k < steps; ++k, ++n_step) {
+            for (int k = 0; k < steps; ++k, ++n_step, v_lo -= kKeys, v_hi -= kKeys, away -= kKeys) {
                 ok = wait_all(&ctrl->s_full, n_step & 1u, kErrS);
                 if (!ok) break;
                 tc_fence_after_sync();
-                const int c0 = first + k * kKeys;
-                const int v_lo = row_lo - c0, v_hi = min(row_hi, hi) - c0;     // keys of this step that the row sees
                 // P with columns of its own: before the first store of P or a rescale of O, the last PV has to be complete (it usually is)
                 auto pv_wait = [&]() {
                     if (!kOwnP || n_step == 0) return true;
@@ -433,9 +459,9 @@ paged_chunk_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Pr
                         for (int i = 0; i < kKeys; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * p.scale_log2);
                     }
                     if (p.slopes != nullptr) {
-                        const float away = (float)(row_hi - 1 - c0);
+                        const float from = (float)away;
 #pragma unroll
-                        for (int i = 0; i < kKeys; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) - slope * (away - (float)i));
+                        for (int i = 0; i < kKeys; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) - slope * (from - (float)i));
                     }
                 }
                 const bool all_there = (present.x & present.y & present.z & present.w) == 0xffffffffu;
@@ -480,34 +506,70 @@ paged_chunk_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Pr
                 if (!ok) break;
                 tc_fence_after_sync();
             }
+            int head;
+            const int token = token_of_row(head), part = x->whole ? -1 : x->part;
             const float inv = l_sum != 0.f ? 1.f / l_sum : 0.f;
+            // O leaves through the memory of the tile's Q rows of this warp, 64 columns in fp32 or 128 in 16 bits at a time, so that stores are whole
+            // lines.  Rows stand as Q's did.
             float2 odd0 = make_float2(0.f, 0.f);
+            const int64_t to = part >= 0 ? ((int64_t)part * kRows + t) * D : token >= 0 ? token * p.o_row + head * p.o_head : -1;
+            const int piece = lane % S::kPieces;
 #pragma unroll
-            for (int ch = 0; ch < D / 32; ++ch) {
-                uint32_t o[32];
+            for (int sub = 0; sub < S::kSub; ++sub) {
+                uint32_t o[64];
                 if (steps > 0) {
-                    tmem_ld32(o_addr + ch * 32, o);
+                    tmem_ld32(o_addr + sub * 64, o);
+                    tmem_ld32(o_addr + sub * 64 + 32, o + 32);
                     tmem_ld_wait();
                 } else {
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) o[i] = 0u;
+                    for (int i = 0; i < 64; ++i) o[i] = 0u;
                 }
 #pragma unroll
-                for (int i = 0; i < 32; i += 2) odd0 = sm::add2(odd0, sm::mul2(make_float2(__uint_as_float(o[i]), __uint_as_float(o[i + 1])), make_float2(0.f, 0.f)));
+                for (int i = 0; i < 64; i += 2) odd0 = sm::fma2(make_float2(__uint_as_float(o[i]), __uint_as_float(o[i + 1])), make_float2(0.f, 0.f), odd0);
                 if (part >= 0) {
-                    float* to = p.part_o + ((int64_t)part * kRows + t) * D + ch * 32;
+                    // 256 bytes to a row: at D = 64 two rows of Q's memory hold one, and the warp's 32 go in two halves
+                    constexpr int kHalves = D == 128 ? 1 : 2;
+                    uint8_t* const stage = smem + warp * 32 * 128;
 #pragma unroll
-                    for (int i = 0; i < 32; i += 4) *reinterpret_cast<uint4*>(to + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
-                } else if (token >= 0) {
-                    T* to = static_cast<T*>(p.o) + token * p.o_row + head * p.o_head + ch * 32;
+                    for (int half = 0; half < kHalves; ++half) {
+                        auto at = [&](int row, int c) {        // 16-byte piece c of the 16 of a row
+                            const int r = kHalves == 1 ? row : (row & 15) * 2 + (c >> 3);
+                            return stage + (kHalves == 1 ? (c >> 3) * S::kSubBytes : 0) + r * 128 + (((c & 7) ^ (row & 7)) << 4);
+                        };
+                        if (kHalves == 1 || (lane >> 4) == half)
 #pragma unroll
-                    for (int i = 0; i < 32; i += 8) {
+                            for (int c = 0; c < 16; ++c) *reinterpret_cast<uint4*>(at(lane, c)) = make_uint4(o[c * 4], o[c * 4 + 1], o[c * 4 + 2], o[c * 4 + 3]);
+                        __syncwarp();
+#pragma unroll
+                        for (int i = 0; i < 32 / kHalves; i += 2) {
+                            const int row = half * 16 + i + (lane >> 4);
+                            const int64_t base = __shfl_sync(0xffffffffu, to, row);
+                            *reinterpret_cast<uint4*>(p.part_o + base + sub * 64 + (lane & 15) * 4) = *reinterpret_cast<const uint4*>(at(row, lane & 15));
+                        }
+                        __syncwarp();
+                    }
+                } else {
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) {
                         uint32_t y[4];
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) y[k] = pack2<T>(__uint_as_float(o[i + 2 * k]) * inv, __uint_as_float(o[i + 2 * k + 1]) * inv);
-                        if (ch * 32 + i < p.d) *reinterpret_cast<uint4*>(to + i) = make_uint4(y[0], y[1], y[2], y[3]);
+                        for (int k = 0; k < 4; ++k) y[k] = pack2<T>(__uint_as_float(o[c * 8 + 2 * k]) * inv, __uint_as_float(o[c * 8 + 2 * k + 1]) * inv);
+                        *reinterpret_cast<uint4*>(smem + sub * S::kSubBytes + t * 128 + ((c ^ (t & 7)) << 4)) = make_uint4(y[0], y[1], y[2], y[3]);
                     }
                 }
+            }
+            if (part < 0) {
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < 32; i += kRowsAtOnce) {
+                    const int row = i + lane / S::kPieces;
+                    const int64_t base = __shfl_sync(0xffffffffu, to, row);
+                    if (base >= 0 && piece * 8 < p.d)
+                        *reinterpret_cast<uint4*>(static_cast<T*>(p.o) + base + piece * 8) =
+                            *reinterpret_cast<const uint4*>(smem + (piece >> 3) * S::kSubBytes + (warp * 32 + row) * 128 + (((piece & 7) ^ (row & 7)) << 4));
+                }
+                __syncwarp();
             }
             if (part >= 0) p.part_rows[(int64_t)part * kRows + t] = make_float4(m_used, l_sum, __int_as_float(token), __int_as_float(head));
             else if (token >= 0 && p.lse != nullptr)
@@ -523,9 +585,9 @@ paged_chunk_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Pr
                     const int from = __ffs(rest) - 1;
                     keys.token = __shfl_sync(0xffffffffu, token, from);
                     keys.head = __shfl_sync(0xffffffffu, head, from);
-                    keys.u = __shfl_sync(0xffffffffu, row_hi, from) - 1;
-                    keys.lo = __shfl_sync(0xffffffffu, row_lo, from);
-                    keys.hi = min(keys.u + 1, hi);
+                    keys.u = x->u0 + p.group.div(x->base + warp * 32 + from);
+                    keys.lo = max(keys.u + 1 - p.taps, x->lo);
+                    keys.hi = min(keys.u + 1, x->hi);
                     keys.slot = (int64_t)part * kRows + warp * 32 + from;
                     row_again<T, D>(p, keys);
                 }
