@@ -542,6 +542,7 @@ extern "C" int32_t splat_paged_attention(const splat_paged_args* args, void* str
     p.scale_log2 = a.scale * kLog2e;
     p.softcap = a.softcap * kLog2e;
     p.cap_inv = a.softcap > 0.f ? a.scale / a.softcap : 0.f;
+    for (int i = 0; i < 7; ++i) p.cap_poly[i] = make_float2(p.softcap * kTanhPoly[i], p.softcap * kTanhPoly[i]);
     p.status = a.status_word;
     p.mirror = a.status_word != nullptr ? status_mirror(a.status_word) : nullptr;
     cudaStream_t st = (cudaStream_t)stream;

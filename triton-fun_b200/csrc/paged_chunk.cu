@@ -452,8 +452,7 @@ paged_chunk_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Pr
                 }
                 if constexpr (kMod) {
                     if (p.softcap > 0.f) {
-#pragma unroll
-                        for (int i = 0; i < kKeys; ++i) r[i] = __float_as_uint(capped(p, __uint_as_float(r[i])));
+                        cap_scores(p, r);
                     } else {
 #pragma unroll
                         for (int i = 0; i < kKeys; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * p.scale_log2);
@@ -495,6 +494,9 @@ paged_chunk_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Pr
                     if (kOwnP && half == 0) ok = pv_wait();
                     tmem_st32(p_addr + half * 32, pk);
                     p_stored(half);
+                    // A branch that is never taken, so that the exponentials of the second half are not moved in front of the first half's
+                    // handing over: 2 x 2048 tokens over 16 k 1228 us without, 1170 with it.
+                    if (half == 0 && p.taps < 1) __nanosleep(20);
                 }
                 l_sum += (acc0.x + acc0.y) + (acc1.x + acc1.y);
                 if (!ok) break;

@@ -50,6 +50,7 @@ struct Problem {
     FastDiv group, stride, page_div;   // query heads per K/V head
     int rows_from, rows_to;            // requests with so many rows in a class are this kernel's
     float scale_log2, softcap, cap_inv;    // x = qk * scale_log2, or softcap_log2 * tanh(qk * cap_inv)
+    float2 cap_poly[7];                // softcap_log2 * tanh(y) / y in powers of y^2, twice each (see paged_rows.cuh)
     // workspace
     int64_t* begins;                   // per CTA: first step of the tile that it begins in the middle of, or -1
     float4* part_rows;                 // [2 per CTA][R] maximum, sum, token, query head
