@@ -10,7 +10,8 @@
 //   * A CTA walks over its share of all steps (paged_schedule.cuh), tile after tile, without a barrier of the block between them: the copying
 //     warp, which alone knows the schedule, runs ahead and hands the others a description of each piece of work through a ring of two.
 //   * K and V come in boxes of 8 to 128 rows, a lane of the copying warp to a box, which also looks up its page.
-//   * Q's rows are (token, head) pairs in any layout: every softmax thread fetches its own.
+//   * Q's rows are (token, head) pairs in any layout: the softmax warps fetch them with cp.async, the next tile's before they write out this
+//     one's O.  (Fetched when the tile begins, through registers: 4 to 10 k cycles of a tile's 3.6 k a step.)
 //   * Keys that a row does not see are masked in S.  Rows of V behind the request's last token, or of a page that is not there, are
 //     set to zero by the copying warp before the multiplication hears of them: what the cache holds there may be NaN as a rule.  Where a
 //     token's own V is not finite, rows that do not see it come out not finite too, are noticed and computed again (row_again).
@@ -289,40 +290,50 @@ paged_chunk_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Pr
             ++n_q;
             if (!ok) break;
             auto half_in = [&](int j, int half) { const int n = first + j * kKeys + half * 64; return n < hi && n + 64 > lo; };
-            auto issue_s = [&](int j, uint32_t step) {
+            uint32_t s_idesc = 0, s_to = 0, s_b = 0;           // of the next S, prepared while P is waited for
+            auto ready_s = [&](int j, uint32_t step) {
                 const int st = step % kSlots;
+                const bool h0 = half_in(j, 0), both = h0 && half_in(j, 1);
+                const uint32_t skip = h0 ? 0u : 1u;
+                s_idesc = both ? idesc_qk : idesc_qk_half;
+                s_to = tmem_base + skip * 64;
+                s_b = k_lo + ((st * S::kTile + skip * 64 * 128) >> 4);
                 ok = wait_all(&ctrl->k_full[st], (step / kSlots) & 1u, kErrKFull);
                 if (ok && kOwnP && step > 0) ok = wait_all(&ctrl->s_free, (step - 1) & 1u, kErrSFree);
-                if (!ok) return;
+            };
+            auto issue_s = [&](uint32_t step) {
                 tc_fence_after_sync();
-                const bool h0 = half_in(j, 0), both = h0 && half_in(j, 1);
-                const uint32_t idesc = both ? idesc_qk : idesc_qk_half, skip = h0 ? 0u : 1u;
                 if (lead) {
-                    const uint32_t to = tmem_base + skip * 64;
-                    const uint32_t b = k_lo + ((st * S::kTile + skip * 64 * 128) >> 4);
 #pragma unroll
                     for (int sub = 0; sub < S::kSub; ++sub)
 #pragma unroll
                         for (int kk = 0; kk < 4; ++kk)
-                            mma_ss(to, desc_sw128(q_lo + ((sub * S::kSubBytes + kk * 32) >> 4)), desc_sw128(b + ((sub * S::kSubBytes + kk * 32) >> 4)), idesc,
+                            mma_ss(s_to, desc_sw128(q_lo + ((sub * S::kSubBytes + kk * 32) >> 4)), desc_sw128(s_b + ((sub * S::kSubBytes + kk * 32) >> 4)), s_idesc,
                                    sub + kk > 0);
                     mma_commit(&ctrl->s_full);
-                    mma_commit(&ctrl->k_free[st]);
+                    mma_commit(&ctrl->k_free[step % kSlots]);
                 }
                 __syncwarp();
             };
-            issue_s(0, n_step);
+            ready_s(0, n_step);
+            if (!ok) break;
+            issue_s(n_step);
             bool first_pv = true;
             for (int j = 0; j < steps && ok; ++j, ++n_step) {
                 if (kOwnP && j + 1 < steps) {                  // the next scores as soon as these have been read
-                    issue_s(j + 1, n_step + 1);
+                    ready_s(j + 1, n_step + 1);
                     if (!ok) break;
+                    issue_s(n_step + 1);
                 }
                 const int st = n_step % kSlots;
                 ok = wait_all(&ctrl->v_full[st], (n_step / kSlots) & 1u, kErrVFull);
                 if (!ok) break;
 #pragma unroll 1
                 for (int half = 0; half < 2; ++half) {
+                    if (!kOwnP && half == 1 && j + 1 < steps) {
+                        ready_s(j + 1, n_step + 1);
+                        if (!ok) break;
+                    }
                     ok = wait_all(&ctrl->p_full[half], n_step & 1u, kErrP);
                     if (!ok) break;
                     tc_fence_after_sync();
@@ -344,7 +355,7 @@ paged_chunk_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Pr
                     if (j + 1 == steps) mma_commit(&ctrl->o_full);
                 }
                 __syncwarp();
-                if (!kOwnP && j + 1 < steps) issue_s(j + 1, n_step + 1);
+                if (!kOwnP && j + 1 < steps) issue_s(n_step + 1);
             }
         }
         // tensor memory is released only after every MMA has completed
@@ -360,21 +371,42 @@ paged_chunk_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Pr
         constexpr int kRowsAtOnce = 32 / S::kPieces;           // of Q and O, in one access of the warp
         const float sc = kMod ? 1.f : p.scale_log2;
         const float2 sc2 = make_float2(sc, sc);
+        // Rows of Q of piece x, once the last tile's products are complete (o_full) and its memory is free: kPieces lanes to a row, 16 bytes each (a lane
+        // to a row touches 32 lines with every load)
+        auto token_of_row = [&](const Piece* x, int& head) {   // of this lane's row, or -1
+            const int m = p.group.div(x->base + t);
+            head = x->head0 + x->base + t - m * (int)p.group.d;
+            return m < x->count ? x->row0 + m * (int)p.stride.d : -1;
+        };
+        auto fetch_q = [&](const Piece* x) {
+            int head;
+            const int token = token_of_row(x, head), piece = lane % S::kPieces;
+            const int64_t from = token >= 0 ? token * p.q_row + head * p.q_head : -1;
+#pragma unroll
+            for (int i = 0; i < 32 / kRowsAtOnce; ++i) {
+                const int row = i * kRowsAtOnce + lane / S::kPieces;
+                const int64_t at = __shfl_sync(0xffffffffu, from, row);
+                const bool there = at >= 0 && piece * 8 < p.d;
+                uint8_t* const to = smem + (piece >> 3) * S::kSubBytes + (warp * 32 + row) * 128 + (((piece & 7) ^ (row & 7)) << 4);
+                const T* const src = static_cast<const T*>(p.q) + (there ? at + piece * 8 : 0);
+                if (q_wide) {
+                    copy16(smem_u32(to), src, there);
+                } else {
+                    __align__(16) T e[8];
+                    for (int k = 0; k < 8; ++k) e[k] = there ? src[k] : DT<T>::from_f(0.f);
+                    *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(e);
+                }
+            }
+        };
         uint32_t n_piece = 0, n_o = 0, n_step = 0;
-        bool ok = true;
+        bool ok = wait_all(&ctrl->piece_full[0], 0, kErrPiece);
+        if (ok && ctrl->piece[0].steps > 0) fetch_q(&ctrl->piece[0]);
         while (ok) {
             const uint32_t slot = n_piece & 1;
-            ok = wait_all(&ctrl->piece_full[slot], (n_piece >> 1) & 1u, kErrPiece);
-            if (!ok) break;
             // (the piece stays until the end of its epilogue; what the loop does not need is read from it again behind it: registers are short)
             const Piece* const x = &ctrl->piece[slot];
             const int steps = x->steps;
             if (steps < 0) break;
-            auto token_of_row = [&](int& head) {               // or -1
-                const int m = p.group.div(x->base + t);
-                head = x->head0 + x->base + t - m * (int)p.group.d;
-                return m < x->count ? x->row0 + m * (int)p.stride.d : -1;
-            };
             int v_lo = 0, v_hi = INT32_MIN / 2, away = 0;      // keys that the row sees, and its own, counted from the step's first
             float slope = 0.f;
             {
@@ -390,34 +422,7 @@ paged_chunk_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Pr
             }
             float m_used = -INFINITY, l_sum = 0.f;
             if (steps > 0) {
-                // Q: the last tile's products are complete (o_full), its memory is free.  kPieces lanes to a row, 16 bytes each (a lane to a row touches 32
-                // lines with every load)
-                int head;
-                const int token = token_of_row(head);
-                const int64_t from = token >= 0 ? token * p.q_row + head * p.q_head : -1;
-                const int piece = lane % S::kPieces;
-                auto q_at = [&](int row) { return smem + (piece >> 3) * S::kSubBytes + (warp * 32 + row) * 128 + (((piece & 7) ^ (row & 7)) << 4); };
-                if (q_wide) {
-                    uint4 v[32 / kRowsAtOnce];                 // (all requested before the first is stored)
-#pragma unroll
-                    for (int i = 0; i < 32 / kRowsAtOnce; ++i) {
-                        const int64_t at = __shfl_sync(0xffffffffu, from, i * kRowsAtOnce + lane / S::kPieces);
-                        const bool there = at >= 0 && piece * 8 < p.d;
-                        v[i] = make_uint4(0, 0, 0, 0);
-                        if (there) v[i] = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + at + piece * 8));
-                    }
-#pragma unroll
-                    for (int i = 0; i < 32 / kRowsAtOnce; ++i) *reinterpret_cast<uint4*>(q_at(i * kRowsAtOnce + lane / S::kPieces)) = v[i];
-                } else {
-#pragma unroll 1
-                    for (int i = 0; i < 32 / kRowsAtOnce; ++i) {
-                        const int64_t at = __shfl_sync(0xffffffffu, from, i * kRowsAtOnce + lane / S::kPieces);
-                        const bool there = at >= 0 && piece * 8 < p.d;
-                        __align__(16) T e[8];
-                        for (int k = 0; k < 8; ++k) e[k] = there ? static_cast<const T*>(p.q)[at + piece * 8 + k] : DT<T>::from_f(0.f);
-                        *reinterpret_cast<uint4*>(q_at(i * kRowsAtOnce + lane / S::kPieces)) = *reinterpret_cast<const uint4*>(e);
-                    }
-                }
+                asm volatile("cp.async.wait_all;" ::: "memory");
                 fence_proxy_async_smem();
                 tc_fence_before_sync();                        // (O of the last tile has been read)
                 __syncwarp();
@@ -509,69 +514,39 @@ paged_chunk_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Pr
                 tc_fence_after_sync();
             }
             int head;
-            const int token = token_of_row(head), part = x->whole ? -1 : x->part;
+            const int token = token_of_row(x, head), part = x->whole ? -1 : x->part;
             const float inv = l_sum != 0.f ? 1.f / l_sum : 0.f;
-            // O leaves through the memory of the tile's Q rows of this warp, 64 columns in fp32 or 128 in 16 bits at a time, so that stores are whole
-            // lines.  Rows stand as Q's did.
+            // The next tile's rows of Q are on their way meanwhile
+            ok = wait_all(&ctrl->piece_full[slot ^ 1], ((n_piece + 1) >> 1) & 1u, kErrPiece);
+            if (!ok) break;
+            if (ctrl->piece[slot ^ 1].steps > 0) fetch_q(&ctrl->piece[slot ^ 1]);
             float2 odd0 = make_float2(0.f, 0.f);
-            const int64_t to = part >= 0 ? ((int64_t)part * kRows + t) * D : token >= 0 ? token * p.o_row + head * p.o_head : -1;
-            const int piece = lane % S::kPieces;
 #pragma unroll
-            for (int sub = 0; sub < S::kSub; ++sub) {
-                uint32_t o[64];
+            for (int ch = 0; ch < D / 32; ++ch) {
+                uint32_t o[32];
                 if (steps > 0) {
-                    tmem_ld32(o_addr + sub * 64, o);
-                    tmem_ld32(o_addr + sub * 64 + 32, o + 32);
+                    tmem_ld32(o_addr + ch * 32, o);
                     tmem_ld_wait();
                 } else {
 #pragma unroll
-                    for (int i = 0; i < 64; ++i) o[i] = 0u;
+                    for (int i = 0; i < 32; ++i) o[i] = 0u;
                 }
 #pragma unroll
-                for (int i = 0; i < 64; i += 2) odd0 = sm::fma2(make_float2(__uint_as_float(o[i]), __uint_as_float(o[i + 1])), make_float2(0.f, 0.f), odd0);
+                for (int i = 0; i < 32; i += 2) odd0 = sm::fma2(make_float2(__uint_as_float(o[i]), __uint_as_float(o[i + 1])), make_float2(0.f, 0.f), odd0);
                 if (part >= 0) {
-                    // 256 bytes to a row: at D = 64 two rows of Q's memory hold one, and the warp's 32 go in two halves
-                    constexpr int kHalves = D == 128 ? 1 : 2;
-                    uint8_t* const stage = smem + warp * 32 * 128;
+                    float* const to = p.part_o + ((int64_t)part * kRows + t) * D + ch * 32;
 #pragma unroll
-                    for (int half = 0; half < kHalves; ++half) {
-                        auto at = [&](int row, int c) {        // 16-byte piece c of the 16 of a row
-                            const int r = kHalves == 1 ? row : (row & 15) * 2 + (c >> 3);
-                            return stage + (kHalves == 1 ? (c >> 3) * S::kSubBytes : 0) + r * 128 + (((c & 7) ^ (row & 7)) << 4);
-                        };
-                        if (kHalves == 1 || (lane >> 4) == half)
+                    for (int i = 0; i < 32; i += 4) *reinterpret_cast<uint4*>(to + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                } else if (token >= 0) {
+                    T* const to = static_cast<T*>(p.o) + token * p.o_row + head * p.o_head + ch * 32;
 #pragma unroll
-                            for (int c = 0; c < 16; ++c) *reinterpret_cast<uint4*>(at(lane, c)) = make_uint4(o[c * 4], o[c * 4 + 1], o[c * 4 + 2], o[c * 4 + 3]);
-                        __syncwarp();
-#pragma unroll
-                        for (int i = 0; i < 32 / kHalves; i += 2) {
-                            const int row = half * 16 + i + (lane >> 4);
-                            const int64_t base = __shfl_sync(0xffffffffu, to, row);
-                            *reinterpret_cast<uint4*>(p.part_o + base + sub * 64 + (lane & 15) * 4) = *reinterpret_cast<const uint4*>(at(row, lane & 15));
-                        }
-                        __syncwarp();
-                    }
-                } else {
-#pragma unroll
-                    for (int c = 0; c < 8; ++c) {
+                    for (int i = 0; i < 32; i += 8) {
                         uint32_t y[4];
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) y[k] = pack2<T>(__uint_as_float(o[c * 8 + 2 * k]) * inv, __uint_as_float(o[c * 8 + 2 * k + 1]) * inv);
-                        *reinterpret_cast<uint4*>(smem + sub * S::kSubBytes + t * 128 + ((c ^ (t & 7)) << 4)) = make_uint4(y[0], y[1], y[2], y[3]);
+                        for (int k = 0; k < 4; ++k) y[k] = pack2<T>(__uint_as_float(o[i + 2 * k]) * inv, __uint_as_float(o[i + 2 * k + 1]) * inv);
+                        if (ch * 32 + i < p.d) *reinterpret_cast<uint4*>(to + i) = make_uint4(y[0], y[1], y[2], y[3]);
                     }
                 }
-            }
-            if (part < 0) {
-                __syncwarp();
-#pragma unroll
-                for (int i = 0; i < 32; i += kRowsAtOnce) {
-                    const int row = i + lane / S::kPieces;
-                    const int64_t base = __shfl_sync(0xffffffffu, to, row);
-                    if (base >= 0 && piece * 8 < p.d)
-                        *reinterpret_cast<uint4*>(static_cast<T*>(p.o) + base + piece * 8) =
-                            *reinterpret_cast<const uint4*>(smem + (piece >> 3) * S::kSubBytes + (warp * 32 + row) * 128 + (((piece & 7) ^ (row & 7)) << 4));
-                }
-                __syncwarp();
             }
             if (part >= 0) p.part_rows[(int64_t)part * kRows + t] = make_float4(m_used, l_sum, __int_as_float(token), __int_as_float(head));
             else if (token >= 0 && p.lse != nullptr)
@@ -598,6 +573,7 @@ paged_chunk_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Pr
             if (lane == 0) mbar_arrive(&ctrl->piece_free[slot]);
             ++n_piece;
         }
+        asm volatile("cp.async.wait_all;" ::: "memory");
     }
     tc_fence_before_sync();
     __syncthreads();

@@ -72,9 +72,6 @@ struct Control {
     int32_t gave_up, stop;
 };
 
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
-}
 // an arrival, one of those that the barrier counts, once all of this thread's copies have landed
 __device__ __forceinline__ void arrive_behind_copies(uint64_t* bar) {
     asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(tc::smem_u32(bar)) : "memory");

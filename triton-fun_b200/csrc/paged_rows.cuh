@@ -27,6 +27,11 @@ __device__ __forceinline__ void load_box(uint32_t smem_dst, const CUtensorMap* m
         : "memory");
 }
 
+// 16 bytes to shared memory, or zeros
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+
 // Row r of a tile: token m of its class, query head of the group.
 template <int R> struct RowPlace {
     int first, last;                   // tokens of the tile (first may be the class's count: no rows)
