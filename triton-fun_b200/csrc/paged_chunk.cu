@@ -89,7 +89,7 @@ template <typename T, int D, bool kMod>
 __global__ void __launch_bounds__(kThreads, kPerSm)
 paged_chunk_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Problem p, const int box, const FastDiv class_page, const bool q_wide) {
     using S = Shape<D>;
-    using Part = Walk<kRows, kKeys, kThreads, kFixed, kSplit>;
+    using Part = Walk<kRows, kKeys, kThreads, kFixed, kSplit, true>;
     constexpr int kSlots = S::kSlots;
     constexpr bool kOwnP = D == 64;                            // P has tensor-memory columns of its own
     constexpr uint32_t kPCol = kOwnP ? kKeys + D : 0;

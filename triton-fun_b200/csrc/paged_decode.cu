@@ -114,7 +114,7 @@ template <typename T, int D, bool kTma>
 __global__ void __launch_bounds__(kThreads, Shape<D>::kPerSm)
 paged_decode_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Problem p, const int box, const FastDiv class_page, const bool q_wide) {
     using S = Shape<D>;
-    using Part = Walk<kRows, S::kKeys, kThreads, kFixed, kSplit>;
+    using Part = Walk<kRows, S::kKeys, kThreads, kFixed, kSplit, false>;
     constexpr int kChunk = S::kChunk;
     extern __shared__ uint8_t smem_raw[];
     __shared__ WalkShared<kThreads> walk;

@@ -38,8 +38,8 @@ template <int R> struct RowPlace {
     int base, g, head0, count, stride;
     int64_t row0;
     FastDiv group;
-    template <int K, int N, int F, int S>
-    __device__ __forceinline__ RowPlace(const Problem& p, const Walk<R, K, N, F, S>& w, const TileRows& t) {
+    template <int K, int N, int F, int S, bool M>
+    __device__ __forceinline__ RowPlace(const Problem& p, const Walk<R, K, N, F, S, M>& w, const TileRows& t) {
         base = w.tile * R;
         g = (int)p.group.d;
         group = p.group;

@@ -105,6 +105,21 @@ __device__ __forceinline__ int64_t cost_of_class(const Problem& p, const Request
     }
     return sum;
 }
+// The same by a warp (the same request in all lanes)
+template <int R, int kKeys, int kFixed>
+__device__ __forceinline__ int64_t cost_by_warp(const Problem& p, const Request& r, int& most) {
+    int64_t sum = 0;
+    for (int t = threadIdx.x & 31; t < r.tiles; t += 32) {
+        const int2 s = steps_of<R, kKeys>(p, r, t);
+        const int cost = s.y - s.x + kFixed;
+        sum += cost;
+        most = max(most, cost);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    most = warp_max_i(most);
+    return sum;
+}
 __device__ __forceinline__ int64_t divide(int64_t a, int64_t b) {
     return ((a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
 }
@@ -115,8 +130,10 @@ template <int kThreads> struct WalkShared {
     int warp_most[kThreads / 32];
 };
 
-// A CTA's walk over its share.  All threads of the block, the same in each.
-template <int R, int kKeys, int kThreads, int kFixed, int kSplit>
+// A CTA's walk over its share.  All threads of the block, the same in each.  kMany: requests have many tiles, and a warp counts those of one
+// together (64 tiles by one thread, three times: 12 us, 2 with a warp.  For the other kernels it is code that does not run and changes how the
+// rest is compiled: 64 ragged requests 85 -> 113 us).
+template <int R, int kKeys, int kThreads, int kFixed, int kSplit, bool kMany>
 struct Walk {
     int64_t end;                       // of the share, in steps and fixed costs of all tiles; or in tiles, which count 1 then
     int64_t tile_begin;                // of the tile
@@ -134,10 +151,28 @@ struct Walk {
         int most = 0;
         for (int i = 0; i < each; ++i) {
             const int q = threadIdx.x * each + i;
-            if (q >= p.requests) break;
-            const Request x = request_of<R>(p, q);
-            cost_mine += cost_of_class<R, kKeys, kFixed>(p, x, most) * x.classes * p.kv_heads;
-            tiles_mine += (int64_t)x.tiles * x.classes * p.kv_heads;
+            if constexpr (kMany) {
+                Request x = {};
+                if (q < p.requests) x = request_of<R>(p, q);
+                const int64_t times = (int64_t)x.classes * p.kv_heads;
+                const bool many = x.tiles > 4;
+                if (!many) cost_mine += cost_of_class<R, kKeys, kFixed>(p, x, most) * times;
+                tiles_mine += x.tiles * times;
+                for (unsigned rest = __ballot_sync(0xffffffffu, many); rest != 0; rest &= rest - 1) {
+                    const int from = __ffs(rest) - 1;
+                    Request y = {};
+                    y.u0 = __shfl_sync(0xffffffffu, x.u0, from);
+                    y.longest = __shfl_sync(0xffffffffu, x.longest, from);
+                    y.tiles = __shfl_sync(0xffffffffu, x.tiles, from);
+                    const int64_t cost = cost_by_warp<R, kKeys, kFixed>(p, y, most);
+                    if (lane == from) cost_mine += cost * times;
+                }
+            } else {
+                if (q >= p.requests) break;
+                const Request x = request_of<R>(p, q);
+                cost_mine += cost_of_class<R, kKeys, kFixed>(p, x, most) * x.classes * p.kv_heads;
+                tiles_mine += (int64_t)x.tiles * x.classes * p.kv_heads;
+            }
         }
         int64_t cost_sum = cost_mine, tiles_sum = tiles_mine;
 #pragma unroll
@@ -176,7 +211,8 @@ struct Walk {
         int64_t sum = sh.before[lo], class_cost;
         for (b = lo * each;; ++b) {    // (ends: what is behind `at` is some request's)
             r = request_of<R>(p, b);
-            class_cost = by_tile ? r.tiles : cost_of_class<R, kKeys, kFixed>(p, r, most);
+            if constexpr (kMany) class_cost = by_tile ? r.tiles : cost_by_warp<R, kKeys, kFixed>(p, r, most);
+            else class_cost = by_tile ? r.tiles : cost_of_class<R, kKeys, kFixed>(p, r, most);
             const int64_t w = class_cost * r.classes * p.kv_heads;
             if (at < sum + w) break;
             sum += w;
@@ -189,6 +225,28 @@ struct Walk {
         rest -= cls * class_cost;
         tile = by_tile ? (int)rest : 0;
         if (by_tile) rest = 0;
+        if constexpr (kMany)
+            for (; !by_tile; tile += 32) {                 // 32 tiles at a time: the one that `rest` is in
+                int x = 0;
+                if (tile + lane < r.tiles) {
+                    const int2 y = steps_of<R, kKeys>(p, r, tile + lane);
+                    x = y.y - y.x + kFixed;
+                }
+                int64_t upto = x;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int64_t y = __shfl_up_sync(0xffffffffu, upto, o);
+                    if (lane >= o) upto += y;
+                }
+                const unsigned behind = __ballot_sync(0xffffffffu, upto > rest);
+                if (behind != 0) {
+                    const int in = __ffs(behind) - 1;
+                    rest -= __shfl_sync(0xffffffffu, upto - x, in);
+                    tile += in;
+                    break;
+                }
+                rest -= __shfl_sync(0xffffffffu, upto, 31);
+            }
         for (;; ++tile) {
             steps = steps_of<R, kKeys>(p, r, tile);
             if (rest < cost()) break;
@@ -230,7 +288,7 @@ struct TileRows {
     int count;                         // tokens of the class
     int u0;                            // index of its first among the class's keys
     int residue;                       // key n of the class is token residue + n * stride
-    template <int R, int K, int N, int F, int S> __device__ __forceinline__ static TileRows of(const Problem& p, const Walk<R, K, N, F, S>& w) {
+    template <int R, int K, int N, int F, int S, bool M> __device__ __forceinline__ static TileRows of(const Problem& p, const Walk<R, K, N, F, S, M>& w) {
         TileRows t;
         const int s = (int)p.stride.d, pos = w.r.pos + w.cls;
         t.count = p.stride.div(w.r.n - w.cls + s - 1);
