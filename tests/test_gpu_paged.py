@@ -284,6 +284,90 @@ def test_many_requests(requests):
     check(batch(F16, lens, 4, 4, 64, 16), scale=0.2)
 
 
+def test_many_requests_with_chunks():
+    rng = random.Random(8)
+    lens = [(rng.randint(20, 60), 20) if rng.random() < 0.7 else (rng.randint(1, 60), 1) for _ in range(300)]
+    check(batch(BF16, lens, 4, 1, 64, 16), scale=0.2)
+    check(batch(F16, [(24, 8)] * 40, 4, 1, 128, 32), scale=0.2, max_q_len=8)
+
+
+def test_a_bound_on_the_lengths_that_does_not_hold():
+    """max_q_len chooses the kernel; requests that bring more, or fewer as the number of rows suggests, are right all the same."""
+    x = batch(BF16, [(300, 150), (40, 1), (70, 9)], 4, 1, 64, 16)
+    want = po.attention(*(x[k] for k in ("q", "k_cache", "v_cache", "block_table", "kv_lens", "q_start")), scale=0.2)
+    for most in (0, 1, 5, 53, 54, 160, 1 << 40):
+        check(x, want=want, scale=0.2, max_q_len=most)
+
+
+def test_cache_without_pages_and_tables_without_columns():
+    x = batch(BF16, [(20, 3), (5, 1)], 4, 2, 64, 16)
+    none = x["k_cache"][:0]
+    out, lse = attend({**x, "k_cache": none, "v_cache": none.clone()})
+    assert bool((out == 0).all()) and bool((lse == float("-inf")).all())
+    out, lse = attend({**x, "block_table": x["block_table"][:, :0].contiguous()})
+    assert bool((out == 0).all()) and bool((lse == float("-inf")).all())
+
+
+def test_large_strides():
+    """Strides and windows beyond every length: a query's own key alone."""
+    x = batch(BF16, [(50, 20), (9, 1)], 4, 2, 64, 16)
+    for kw in (dict(stride=1 << 40), dict(taps=1), dict(stride=2 ** 31, taps=2 ** 40)):
+        check(x, scale=0.2, **({"stride": 1 << 20} if "taps" not in kw else {"taps": 1}))
+        a, b = attend(x, scale=0.2, **kw), attend(x, scale=0.2, taps=1)
+        assert torch.equal(a[0], b[0])
+    check(x, scale=0.2, taps=2 ** 40)
+
+
+@pytest.mark.parametrize("heads, kv_heads", [(64, 1), (130, 2), (33, 3)])
+def test_many_heads_to_a_group(heads, kv_heads):
+    check(batch(F16, [(200, 1), (40, 3)], heads, kv_heads, 64, 16), scale=0.2)
+
+
+def test_a_reported_wait_stops_the_kernels_and_is_raised():
+    """While the status word is set the tensor-core kernels do nothing; the next call raises and clears it."""
+    import splat_native as n
+    dev = torch.device("cuda", torch.cuda.current_device())
+    x, y = batch(BF16, [(200, 1)], 4, 2, 64, 16), batch(BF16, [(200, 100)], 4, 2, 64, 16)
+    attend(x), attend(y)
+    for z, kw in ((x, dict(max_q_len=1)), (y, {})):
+        n.status_word(dev).fill_(81)
+        torch.cuda.synchronize()
+        out, lse = attend(z, **kw)
+        torch.cuda.synchronize()
+        assert bool((out == 7).all()) and bool((lse == 7).all())
+        with pytest.raises(RuntimeError, match="code 81"):
+            attend(z, **kw)
+        check(z, scale=0.2, **kw)
+
+
+def test_first_call_of_a_process_is_captured():
+    """No status word yet, and none can be set up: kernels without bounded waits run, with the same results."""
+    import os
+    import subprocess
+    import sys
+    import textwrap
+    from conftest import ROOT, SPLAT_DIR
+    code = """
+        import torch
+        import test_gpu_paged as t
+        from oracle import paged_oracle as po
+        for lens in ([(300, 1), (40, 1)], [(200, 90), (30, 3)]):
+            x = t.batch(torch.bfloat16, lens, 4, 2, 64, 16)
+            out = torch.full(x["q"].shape, 7.0, device="cuda", dtype=x["q"].dtype)
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                t.r_paged.rpaged_attention_launcher(x["q"], x["k_cache"], x["v_cache"], x["block_table"], x["kv_lens"], out,
+                                                    q_start=x["q_start"], scale=0.2)
+            graph.replay()
+            want, _, tol, _ = po.attention(*(x[k] for k in ("q", "k_cache", "v_cache", "block_table", "kv_lens", "q_start")), scale=0.2)
+            assert bool(((out.double() - want).abs() <= tol).all())
+        print("alive")
+        """
+    head = f"import sys; sys.path[:0] = [{ROOT!r}, {SPLAT_DIR!r}, {os.path.join(ROOT, 'tests')!r}]\n"
+    r = subprocess.run([sys.executable, "-c", head + textwrap.dedent(code)], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "alive" in r.stdout, r.stderr[-2000:]
+
+
 def test_results_do_not_depend_on_timing():
     x = batch(BF16, [(9000, 1), (5000, 200), (17, 1)], 8, 2, 128, 16)
     first = attend(x, scale=0.1)
