@@ -472,7 +472,7 @@ int box_rows(const splat_paged_args& a, int most) {
     const int box = (int)(power < most ? power : most);
     return box >= 8 ? box : 0;
 }
-bool cache_map(CUtensorMap* map, const splat_paged_args& a, const void* base, int64_t page, int64_t head, int64_t row, int rows) {
+static bool encode(CUtensorMap* map, const splat_paged_args& a, int rank, const void* base, const cuuint64_t* dims, cuuint64_t* strides, const cuuint32_t* box) {
     static const EncodeTiledFn fn = [] {
         void* f = nullptr;
         cudaDriverEntryPointQueryResult q;
@@ -480,17 +480,26 @@ bool cache_map(CUtensorMap* map, const splat_paged_args& a, const void* base, in
         return reinterpret_cast<EncodeTiledFn>(f);
     }();
     if (fn == nullptr) return false;
-    const int64_t class_rows = a.page / a.stride;
-    const cuuint64_t dims[5] = {(cuuint64_t)a.d, (cuuint64_t)a.stride, (cuuint64_t)class_rows, (cuuint64_t)a.kv_heads, (cuuint64_t)a.pages};
-    cuuint64_t strides[4] = {(cuuint64_t)(row * 2), (cuuint64_t)(a.stride * row * 2), (cuuint64_t)(head * 2), (cuuint64_t)(page * 2)};
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i + 1 < rank; ++i) {
         if (dims[i + 1] == 1) strides[i] = (cuuint64_t)(a.d * 2);      // (never stepped over)
-        if (strides[i] == 0) return false;                             // an expanded cache
+        if (strides[i] == 0) return false;                             // an expanded tensor
     }
-    const cuuint32_t box[5] = {64, 1, (cuuint32_t)rows, 1, 1}, each[5] = {1, 1, 1, 1, 1};
-    return fn(map, a.dtype == SPLAT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5, const_cast<void*>(base), dims, strides,
-              box, each, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+    const cuuint32_t each[5] = {1, 1, 1, 1, 1};
+    return fn(map, a.dtype == SPLAT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, (cuuint32_t)rank, const_cast<void*>(base),
+              dims, strides, box, each, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+bool cache_map(CUtensorMap* map, const splat_paged_args& a, const void* base, int64_t page, int64_t head, int64_t row, int rows) {
+    const cuuint64_t dims[5] = {(cuuint64_t)a.d, (cuuint64_t)a.stride, (cuuint64_t)(a.page / a.stride), (cuuint64_t)a.kv_heads, (cuuint64_t)a.pages};
+    cuuint64_t strides[4] = {(cuuint64_t)(row * 2), (cuuint64_t)(a.stride * row * 2), (cuuint64_t)(head * 2), (cuuint64_t)(page * 2)};
+    const cuuint32_t box[5] = {64, 1, (cuuint32_t)rows, 1, 1};
+    return encode(map, a, 5, base, dims, strides, box);
+}
+bool rows_map(CUtensorMap* map, const splat_paged_args& a, int heads, int tokens) {
+    const cuuint64_t dims[3] = {(cuuint64_t)a.d, (cuuint64_t)a.heads, (cuuint64_t)a.tokens};
+    cuuint64_t strides[2] = {(cuuint64_t)(a.q_head * 2), (cuuint64_t)(a.q_row * 2)};
+    const cuuint32_t box[3] = {64, (cuuint32_t)heads, (cuuint32_t)tokens};
+    return encode(map, a, 3, a.q, dims, strides, box);
 }
 
 // paged_decode.cu, paged_chunk.cu (which may answer SPLAT_ERR_UNSUPPORTED_SHAPE, and has then launched nothing)

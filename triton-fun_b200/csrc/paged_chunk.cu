@@ -10,8 +10,10 @@
 //   * A CTA walks over its share of all steps (paged_schedule.cuh), tile after tile, without a barrier of the block between them: the copying
 //     warp, which alone knows the schedule, runs ahead and hands the others a description of each piece of work through a ring of two.
 //   * K and V come in boxes of 8 to 128 rows, a lane of the copying warp to a box, which also looks up its page.
-//   * Q's rows are (token, head) pairs in any layout: the softmax warps fetch them with cp.async, the next tile's before they write out this
-//     one's O.  (Fetched when the tile begins, through registers: 4 to 10 k cycles of a tile's 3.6 k a step.)
+//   * Q's rows are (token, head) pairs.  Where the tile is whole tokens (a group of 2^n heads, stride 1) they are a box of a 3-D map and come
+//     by a tiled copy as soon as the last tile's scores are complete, so that the next tile's first scores are formed while this one's O is
+//     written out; otherwise the softmax warps fetch them, with cp.async, before they write out O.  (Fetched through registers when
+//     the tile begins: 4 to 10 k cycles, where a step takes 3.6 k.)
 //   * Keys that a row does not see are masked in S.  Rows of V behind the request's last token, or of a page that is not there, are
 //     set to zero by the copying warp before the multiplication hears of them: what the cache holds there may be NaN as a rule.  Where a
 //     token's own V is not finite, rows that do not see it come out not finite too, are noticed and computed again (row_again).
@@ -37,9 +39,9 @@ constexpr int kFixed = 3;                       // what a tile costs beside its 
 constexpr int kSplit = 6;                       // what dividing one costs
 constexpr int kTmemCols = 256, kPerSm = 2;
 constexpr float kLazy = 8.f;                    // log2: the maximum is raised when it has grown by more
-enum : int { kErrPiece = 91, kErrPieceFree, kErrQ, kErrKFull, kErrKFree, kErrVFull, kErrVFree, kErrVLanded, kErrS, kErrSFree, kErrP, kErrPv, kErrO };
+enum : int { kErrPiece = 91, kErrPieceFree, kErrQ, kErrQFree, kErrOFree, kErrKFull, kErrKFree, kErrVFull, kErrVFree, kErrVLanded, kErrS, kErrSFree, kErrP, kErrPv, kErrO };
 
-struct Maps { CUtensorMap k, v; };
+struct Maps { CUtensorMap k, v, q; };
 
 template <int D> struct Shape {
     static constexpr int kSub = D / 64, kPieces = D / 8;       // boxes of 64 columns; 16-byte pieces of a row
@@ -61,7 +63,7 @@ struct Piece {                                  // of a tile: what the softmax w
 
 struct Control {
     uint64_t piece_full[2], piece_free[2];
-    uint64_t q_full, o_full, drain, v_landed;
+    uint64_t q_full, q_free, o_full, o_free, drain, v_landed;
     uint64_t k_full[2], k_free[2], v_full[2], v_free[2];
     uint64_t s_full, s_free, p_full[2], pv_done;
     Piece piece[2];
@@ -87,7 +89,7 @@ __device__ __forceinline__ void rescale_o(uint32_t o_addr, int n, float corr) {
 // kMod: scores are capped, biased or multiplied by a scale that is not positive, one by one, before the maximum is taken.
 template <typename T, int D, bool kMod>
 __global__ void __launch_bounds__(kThreads, kPerSm)
-paged_chunk_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Problem p, const int box, const FastDiv class_page, const bool q_wide) {
+paged_chunk_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Problem p, const int box, const FastDiv class_page, const bool q_wide, const bool q_tma) {
     using S = Shape<D>;
     using Part = Walk<kRows, kKeys, kThreads, kFixed, kSplit, true>;
     constexpr int kSlots = S::kSlots;
@@ -109,7 +111,9 @@ paged_chunk_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Pr
             mbar_init(&ctrl->v_free[i], 1);
             mbar_init(&ctrl->p_full[i], 4);
         }
-        mbar_init(&ctrl->q_full, 4);
+        mbar_init(&ctrl->q_full, q_tma ? 1 : 4);
+        mbar_init(&ctrl->q_free, 1);
+        mbar_init(&ctrl->o_free, 4);
         mbar_init(&ctrl->o_full, 1);
         mbar_init(&ctrl->drain, 1);
         mbar_init(&ctrl->v_landed, 1);
@@ -119,6 +123,7 @@ paged_chunk_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Pr
         mbar_fence_init();
         tma_prefetch_desc(&maps.k);
         tma_prefetch_desc(&maps.v);
+        if (q_tma) tma_prefetch_desc(&maps.q);
     }
     depend_wait();
     if (threadIdx.x == 0) {
@@ -146,7 +151,7 @@ paged_chunk_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Pr
 
     if (warp == kTmaWarp) {
         // ------------------------------------------------------------------ schedule and copies
-        uint32_t n_piece = 0, n_step = 0, n_edge = 0;          // pieces, steps, and steps with rows to be set to zero, so far
+        uint32_t n_piece = 0, n_q = 0, n_step = 0, n_edge = 0; // pieces, those with steps, steps, and steps with rows to be set to zero, so far
         uint32_t k_issued = 0, v_issued = 0;                   // (for the way out)
         const int s = (int)p.stride.d;
         bool ok = true, more = true;
@@ -176,7 +181,18 @@ paged_chunk_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Pr
             const int head = w.head, limit = t.u0 + t.count;   // keys of the class
             const int32_t* table = p.table + w.b * p.table_stride;
             hand_over(x);
-            if (x.steps > 0) {                                 // its rows of Q, to the L2 cache by the time that they are asked for
+            if (!ok) break;
+            if (x.steps > 0 && q_tma) {                        // its rows of Q, once the last tile's scores are complete
+                if (n_q > 0) ok = wait_all(&ctrl->q_free, (n_q - 1) & 1u, kErrQFree);
+                if (!ok) break;
+                if (lane == 0) {
+                    mbar_arrive_expect_tx(&ctrl->q_full, S::kTile);
+                    for (int sub = 0; sub < S::kSub; ++sub)
+                        tma_load_3d(smem + sub * S::kSubBytes, &maps.q, &ctrl->q_full, sub * 64, x.head0, x.row0 + p.group.div(x.base));
+                }
+                __syncwarp();
+                ++n_q;
+            } else if (x.steps > 0) {                          // ... or to the L2 cache by the time that they are asked for
                 for (int r = lane; r < kRows; r += 32) {
                     const int m = rows.token_of(r);
                     if (m < 0) continue;
@@ -262,6 +278,7 @@ paged_chunk_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Pr
             hand_over(end);
         }
         if (!ok) {                                             // leave only after the copies already issued have landed
+            if (q_tma && n_q > 0) wait_quiet(&ctrl->q_full, (n_q - 1) & 1u);
             for (uint32_t i = k_issued > kSlots ? k_issued - kSlots : 0; i < k_issued; ++i) wait_quiet(&ctrl->k_full[i % kSlots], (i / kSlots) & 1u);
             for (uint32_t i = v_issued > kSlots ? v_issued - kSlots : 0; i < v_issued; ++i) wait_quiet(&ctrl->v_full[i % kSlots], (i / kSlots) & 1u);
         }
@@ -286,7 +303,7 @@ paged_chunk_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Pr
             ++n_piece;
             if (steps < 0) break;
             if (steps == 0) continue;
-            ok = wait_all(&ctrl->q_full, n_q & 1u, kErrQ);     // (which comes behind the reading of the last tile's O)
+            ok = wait_all(&ctrl->q_full, n_q & 1u, kErrQ);
             ++n_q;
             if (!ok) break;
             auto half_in = [&](int j, int half) { const int n = first + j * kKeys + half * 64; return n < hi && n + 64 > lo; };
@@ -301,7 +318,7 @@ paged_chunk_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Pr
                 ok = wait_all(&ctrl->k_full[st], (step / kSlots) & 1u, kErrKFull);
                 if (ok && kOwnP && step > 0) ok = wait_all(&ctrl->s_free, (step - 1) & 1u, kErrSFree);
             };
-            auto issue_s = [&](uint32_t step) {
+            auto issue_s = [&](uint32_t step, bool last) {
                 tc_fence_after_sync();
                 if (lead) {
 #pragma unroll
@@ -312,21 +329,23 @@ paged_chunk_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Pr
                                    sub + kk > 0);
                     mma_commit(&ctrl->s_full);
                     mma_commit(&ctrl->k_free[step % kSlots]);
+                    if (last) mma_commit(&ctrl->q_free);
                 }
                 __syncwarp();
             };
             ready_s(0, n_step);
             if (!ok) break;
-            issue_s(n_step);
+            issue_s(n_step, steps == 1);
             bool first_pv = true;
             for (int j = 0; j < steps && ok; ++j, ++n_step) {
                 if (kOwnP && j + 1 < steps) {                  // the next scores as soon as these have been read
                     ready_s(j + 1, n_step + 1);
                     if (!ok) break;
-                    issue_s(n_step + 1);
+                    issue_s(n_step + 1, j + 2 == steps);
                 }
                 const int st = n_step % kSlots;
                 ok = wait_all(&ctrl->v_full[st], (n_step / kSlots) & 1u, kErrVFull);
+                if (ok && j == 0 && n_q > 1) ok = wait_all(&ctrl->o_free, (n_q - 2) & 1u, kErrOFree);      // the last tile's O has been read
                 if (!ok) break;
 #pragma unroll 1
                 for (int half = 0; half < 2; ++half) {
@@ -355,7 +374,7 @@ paged_chunk_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Pr
                     if (j + 1 == steps) mma_commit(&ctrl->o_full);
                 }
                 __syncwarp();
-                if (!kOwnP && j + 1 < steps) issue_s(n_step + 1);
+                if (!kOwnP && j + 1 < steps) issue_s(n_step + 1, j + 2 == steps);
             }
         }
         // tensor memory is released only after every MMA has completed
@@ -382,7 +401,9 @@ paged_chunk_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Pr
             int head;
             const int token = token_of_row(x, head), piece = lane % S::kPieces;
             const int64_t from = token >= 0 ? token * p.q_row + head * p.q_head : -1;
-#pragma unroll
+            // (not unrolled, nor is the loop over O below: code that runs once in a tile comes from beyond the instruction cache, 5 cycles and more an
+            // instruction.  85 prompts of 451 tokens, 32 / 4 heads, d96 481 us unrolled)
+#pragma unroll 2
             for (int i = 0; i < 32 / kRowsAtOnce; ++i) {
                 const int row = i * kRowsAtOnce + lane / S::kPieces;
                 const int64_t at = __shfl_sync(0xffffffffu, from, row);
@@ -393,16 +414,21 @@ paged_chunk_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Pr
                     copy16(smem_u32(to), src, there);
                 } else {
                     __align__(16) T e[8];
+#pragma unroll 1
                     for (int k = 0; k < 8; ++k) e[k] = there ? src[k] : DT<T>::from_f(0.f);
                     *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(e);
                 }
             }
         };
         uint32_t n_piece = 0, n_o = 0, n_step = 0;
-        bool ok = wait_all(&ctrl->piece_full[0], 0, kErrPiece);
-        if (ok && ctrl->piece[0].steps > 0) fetch_q(&ctrl->piece[0]);
+        bool ok = q_tma || wait_all(&ctrl->piece_full[0], 0, kErrPiece);
+        if (ok && !q_tma && ctrl->piece[0].steps > 0) fetch_q(&ctrl->piece[0]);
         while (ok) {
             const uint32_t slot = n_piece & 1;
+            if (q_tma) {                                       // (otherwise it has been waited for, for its rows of Q)
+                ok = wait_all(&ctrl->piece_full[slot], (n_piece >> 1) & 1u, kErrPiece);
+                if (!ok) break;
+            }
             // (the piece stays until the end of its epilogue; what the loop does not need is read from it again behind it: registers are short)
             const Piece* const x = &ctrl->piece[slot];
             const int steps = x->steps;
@@ -421,10 +447,9 @@ paged_chunk_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Pr
                 }
             }
             float m_used = -INFINITY, l_sum = 0.f;
-            if (steps > 0) {
+            if (steps > 0 && !q_tma) {
                 asm volatile("cp.async.wait_all;" ::: "memory");
                 fence_proxy_async_smem();
-                tc_fence_before_sync();                        // (O of the last tile has been read)
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&ctrl->q_full);
             }
@@ -516,12 +541,13 @@ paged_chunk_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Pr
             int head;
             const int token = token_of_row(x, head), part = x->whole ? -1 : x->part;
             const float inv = l_sum != 0.f ? 1.f / l_sum : 0.f;
-            // The next tile's rows of Q are on their way meanwhile
-            ok = wait_all(&ctrl->piece_full[slot ^ 1], ((n_piece + 1) >> 1) & 1u, kErrPiece);
-            if (!ok) break;
-            if (ctrl->piece[slot ^ 1].steps > 0) fetch_q(&ctrl->piece[slot ^ 1]);
+            if (!q_tma) {                                      // the next tile's rows of Q are on their way meanwhile
+                ok = wait_all(&ctrl->piece_full[slot ^ 1], ((n_piece + 1) >> 1) & 1u, kErrPiece);
+                if (!ok) break;
+                if (ctrl->piece[slot ^ 1].steps > 0) fetch_q(&ctrl->piece[slot ^ 1]);
+            }
             float2 odd0 = make_float2(0.f, 0.f);
-#pragma unroll
+#pragma unroll 1
             for (int ch = 0; ch < D / 32; ++ch) {
                 uint32_t o[32];
                 if (steps > 0) {
@@ -547,6 +573,11 @@ paged_chunk_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Pr
                         if (ch * 32 + i < p.d) *reinterpret_cast<uint4*>(to + i) = make_uint4(y[0], y[1], y[2], y[3]);
                     }
                 }
+            }
+            if (steps > 0) {                                   // the next tile's products may be added up
+                tc_fence_before_sync();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&ctrl->o_free);
             }
             if (part >= 0) p.part_rows[(int64_t)part * kRows + t] = make_float4(m_used, l_sum, __int_as_float(token), __int_as_float(head));
             else if (token >= 0 && p.lse != nullptr)
@@ -586,11 +617,11 @@ paged_chunk_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Pr
 }
 
 template <typename T, int D>
-static int32_t launch(const Problem& p, int ctas, const Maps& maps, int box, FastDiv class_page, bool q_wide, cudaStream_t st) {
+static int32_t launch(const Problem& p, int ctas, const Maps& maps, int box, FastDiv class_page, bool q_wide, bool q_tma, cudaStream_t st) {
     const bool mod = p.softcap > 0.f || p.slopes != nullptr || !(p.scale_log2 > 0.f);
     auto kern = mod ? paged_chunk_kernel<T, D, true> : paged_chunk_kernel<T, D, false>;
     if (!band::allow_dynamic_smem(reinterpret_cast<const void*>(kern), Shape<D>::kSmem)) return SPLAT_ERR_LAUNCH;
-    return launch_kernel(kern, dim3((unsigned)ctas), dim3(kThreads), Shape<D>::kSmem, st, maps, p, box, class_page, q_wide);
+    return launch_kernel(kern, dim3((unsigned)ctas), dim3(kThreads), Shape<D>::kSmem, st, maps, p, box, class_page, q_wide, q_tma);
 }
 
 }  // namespace chunk
@@ -607,9 +638,12 @@ int32_t attend_chunk(const splat_paged_args& a, Problem p, int sms, void* worksp
     paged::Layout(ctas, kRows, d_pad).place(p, workspace);
     const FastDiv class_page((uint32_t)(a.page / a.stride));
     const bool q_wide = aligned16(a.q) && a.q_row % 8 == 0 && a.q_head % 8 == 0;
+    const int64_t group = a.heads / a.kv_heads;
+    const bool q_tma = q_wide && a.stride == 1 && kRows % group == 0 && rows_map(&maps.q, a, (int)group, (int)(kRows / group));
     auto run = [&](auto element) {
         using T = decltype(element);
-        return d_pad == 64 ? launch<T, 64>(p, ctas, maps, box, class_page, q_wide, st) : launch<T, 128>(p, ctas, maps, box, class_page, q_wide, st);
+        return d_pad == 64 ? launch<T, 64>(p, ctas, maps, box, class_page, q_wide, q_tma, st)
+                           : launch<T, 128>(p, ctas, maps, box, class_page, q_wide, q_tma, st);
     };
     const int32_t rc = a.dtype == SPLAT_BF16 ? run(__nv_bfloat16()) : run(__half());
     return rc != SPLAT_OK ? rc : join_parts(p, ctas, kRows, d_pad, a.dtype, st);

@@ -19,12 +19,21 @@ int box_rows(const splat_paged_args& a, int most);
 // The cache as (columns, residues, rows of a class in a page, heads, pages), boxes of 64 columns and `rows` rows.  False if it cannot be
 // described so.  Both in paged_attention.cu.
 bool cache_map(CUtensorMap* map, const splat_paged_args& a, const void* base, int64_t page, int64_t head, int64_t row, int rows);
+// q as (columns, heads, tokens), boxes of 64 columns.
+bool rows_map(CUtensorMap* map, const splat_paged_args& a, int heads, int tokens);
 
 __device__ __forceinline__ void load_box(uint32_t smem_dst, const CUtensorMap* map, uint64_t* bar, int column, int residue, int row, int head, int page) {
     asm volatile(
         "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], [%2];" ::"r"(smem_dst),
         "l"(map), "r"(tc::smem_u32(bar)), "r"(column), "r"(residue), "r"(row), "r"(head), "r"(page)
         : "memory");
+}
+
+__device__ __forceinline__ void tma_load_3d(void* smem_dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1, int c2) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(
+                     tc::smem_u32(smem_dst)),
+                 "l"(map), "r"(tc::smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
+                 : "memory");
 }
 
 // 16 bytes to shared memory, or zeros
