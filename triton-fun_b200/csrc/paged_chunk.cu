@@ -49,7 +49,8 @@ template <int D> struct Shape {
     static constexpr int kTile = kSub * kSubBytes;             // Q, or a step's K or V
     static constexpr int kSlots = D == 128 ? 1 : 2;            // steps of K, and of V
     static constexpr int kKOff = kTile, kVOff = kKOff + kSlots * kTile;
-    static constexpr int kSmem = kVOff + kSlots * kTile + 1024;        // + alignment slack
+    static constexpr int kStageOff = kVOff + kSlots * kTile;   // 64 bytes of each row of O, on their way out
+    static constexpr int kSmem = kStageOff + kRows * 64 + 1024;        // + alignment slack
 };
 
 struct Piece {                                  // of a tile: what the softmax warps and the issuer have to know
@@ -546,7 +547,12 @@ paged_chunk_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Pr
                 if (!ok) break;
                 if (ctrl->piece[slot ^ 1].steps > 0) fetch_q(&ctrl->piece[slot ^ 1]);
             }
+            // O leaves in pieces of 64 bytes of each of the warp's rows, through shared memory: four lanes to a row's piece, eight lines to a store (a lane to
+            // a row is 32, and 3 to 4 k cycles to a tile)
             float2 odd0 = make_float2(0.f, 0.f);
+            const int64_t to = part >= 0 ? ((int64_t)part * kRows + t) * D : token >= 0 ? token * p.o_row + head * p.o_head : -1;
+            uint8_t* const stage = smem + S::kStageOff + warp * 32 * 64;
+            auto place = [&](int row, int piece) { return reinterpret_cast<uint4*>(stage + row * 64 + ((piece ^ ((row >> 1) & 3)) << 4)); };
 #pragma unroll 1
             for (int ch = 0; ch < D / 32; ++ch) {
                 uint32_t o[32];
@@ -560,18 +566,35 @@ paged_chunk_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Pr
 #pragma unroll
                 for (int i = 0; i < 32; i += 2) odd0 = sm::fma2(make_float2(__uint_as_float(o[i]), __uint_as_float(o[i + 1])), make_float2(0.f, 0.f), odd0);
                 if (part >= 0) {
-                    float* const to = p.part_o + ((int64_t)part * kRows + t) * D + ch * 32;
 #pragma unroll
-                    for (int i = 0; i < 32; i += 4) *reinterpret_cast<uint4*>(to + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
-                } else if (token >= 0) {
-                    T* const to = static_cast<T*>(p.o) + token * p.o_row + head * p.o_head + ch * 32;
+                    for (int half = 0; half < 2; ++half) {
 #pragma unroll
-                    for (int i = 0; i < 32; i += 8) {
+                        for (int c = 0; c < 4; ++c)
+                            *place(lane, c) = make_uint4(o[half * 16 + c * 4], o[half * 16 + c * 4 + 1], o[half * 16 + c * 4 + 2], o[half * 16 + c * 4 + 3]);
+                        __syncwarp();
+#pragma unroll
+                        for (int i = 0; i < 32; i += 8) {
+                            const int64_t at = __shfl_sync(0xffffffffu, to, i + (lane >> 2));
+                            *reinterpret_cast<uint4*>(p.part_o + at + ch * 32 + half * 16 + (lane & 3) * 4) = *place(i + (lane >> 2), lane & 3);
+                        }
+                        __syncwarp();
+                    }
+                } else {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
                         uint32_t y[4];
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) y[k] = pack2<T>(__uint_as_float(o[i + 2 * k]) * inv, __uint_as_float(o[i + 2 * k + 1]) * inv);
-                        if (ch * 32 + i < p.d) *reinterpret_cast<uint4*>(to + i) = make_uint4(y[0], y[1], y[2], y[3]);
+                        for (int k = 0; k < 4; ++k) y[k] = pack2<T>(__uint_as_float(o[c * 8 + 2 * k]) * inv, __uint_as_float(o[c * 8 + 2 * k + 1]) * inv);
+                        *place(lane, c) = make_uint4(y[0], y[1], y[2], y[3]);
                     }
+                    __syncwarp();
+#pragma unroll
+                    for (int i = 0; i < 32; i += 8) {
+                        const int64_t at = __shfl_sync(0xffffffffu, to, i + (lane >> 2));
+                        const int col = ch * 32 + (lane & 3) * 8;
+                        if (at >= 0 && col < p.d) *reinterpret_cast<uint4*>(static_cast<T*>(p.o) + at + col) = *place(i + (lane >> 2), lane & 3);
+                    }
+                    __syncwarp();
                 }
             }
             if (steps > 0) {                                   // the next tile's products may be added up
