@@ -150,11 +150,14 @@ PyObject* paged_tables(PyObject* const* a, Py_ssize_t n) {
     rows_contiguous(table);
     if (B > 1 && table->stride(0) < table->size(1)) refuse("block_table: its rows must not overlap");
     const int dev = device_of({ctx, fresh, table, ring, span, kv, start, slots, positions, requests, taken});
-    for (const Operand* out : {&table, &kv, &start, &slots, &positions, &requests, &taken}) {
-        for (const Operand* in : {&ctx, &fresh, &ring, &span}) distinct(*out, *in);
-        for (const Operand* other : {&table, &kv, &start, &slots, &positions, &requests, &taken})
-            if (other != out) distinct(*out, *other);
-    }
+    // outputs may be nobody else's memory (addresses first: asking the tensors for each pair takes longer than the launch)
+    const Operand* const all[] = {&table, &kv, &start, &slots, &positions, &requests, &taken, &ctx, &fresh, &ring, &span};
+    constexpr int kOutputs = 7, kAll = 11;
+    const void* at[kAll];
+    for (int i = 0; i < kAll; ++i) at[i] = (*all[i])->numel() > 0 ? (*all[i])->const_data_ptr() : nullptr;
+    for (int i = 0; i < kOutputs; ++i)
+        for (int j = i + 1; j < kAll; ++j)
+            if (at[i] != nullptr && at[i] == at[j]) distinct(*all[i], *all[j]);
     c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(dev));
     check(g_tables(data<int32_t>(ctx), data<int32_t>(fresh), data<int32_t>(table), B > 1 ? table->stride(0) : table->size(1),
                    data<int32_t>(ring), ring->size(0), data<int64_t>(span), page, B, table->size(1), T, data<int32_t>(kv),

@@ -35,8 +35,8 @@ using sm::ex2;
 using sm::pack2;
 
 constexpr int kRows = 128, kKeys = 128, kThreads = 192, kTmaWarp = 4, kMmaWarp = 5;
-constexpr int kFixed = 3;                       // what a tile costs beside its steps, in steps
-constexpr int kSplit = 6;                       // what dividing one costs
+constexpr int kFixed = 2;                       // what a tile costs beside its steps, in steps
+constexpr int kSplit = 8;                       // what dividing one costs
 constexpr int kTmemCols = 256, kPerSm = 2;
 constexpr float kLazy = 8.f;                    // log2: the maximum is raised when it has grown by more
 enum : int { kErrPiece = 91, kErrPieceFree, kErrQ, kErrQFree, kErrOFree, kErrKFull, kErrKFree, kErrVFull, kErrVFree, kErrVLanded, kErrS, kErrSFree, kErrP, kErrPv, kErrO };
