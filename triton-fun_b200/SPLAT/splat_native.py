@@ -23,14 +23,14 @@ if not os.path.exists(LIB_PATH):
 
 _lib = ctypes.CDLL(LIB_PATH)
 try:
-    import splat_host as _host      # native host path of the launchers (csrc/host_binding.cpp)
+    import splat_host as _host      # native host path of the launchers (csrc/host_binding.cpp, paged_binding.cpp)
 except ImportError as e:
     raise ImportError(f"the splat_host extension is missing or does not load ({e}): build it with "
                       f"`python {os.path.join(_PKG_DIR, 'build.py')}`") from e
 
 _i32, _i64, _f32, _vp = ctypes.c_int32, ctypes.c_int64, ctypes.c_float, ctypes.c_void_p
 
-# name -> argtypes; every function returns int32 except splat_status_string
+# name -> argtypes; every function returns int32 except splat_status_string and splat_paged_attention_workspace
 SIGNATURES = {
     "splat_version": [],
     "splat_mask_row_summary_u8": [_vp, _i64, _i64, _i64, _vp, _vp],

@@ -22,7 +22,8 @@ __device__ __forceinline__ float score_of(const Problem& p, float dot) {
 // A tile is R rows: 8, or 4 or 2 where no request can have more.  kLanes lanes (16 for d <= 64, else the warp) hold a key: each has kCols of
 // its columns and of the rows' q and o.  The R dot products are added up over the lanes by halving: with 8 rows 4 + 2 + 1 exchanges leave
 // every lane with one row's sum over some lanes, one or two more complete it (8 to 9 shuffles for 8 sums; one by one they would be 32 to 40).
-// Issue slots bound it: a key is 22 cycles of HBM (d64), or 89 issue slots, and takes some 54 with 8 rows.  A block's 4 warps are 4 or 8 streams that
+// Issue slots bound it (56 % busy, HBM 64 %): 32 requests of 4096 tokens, 32 / 8 heads, d128 fp32 257 us, 4.2 TB/s; without the next keys on
+// their way 519.  A block's 4 warps are 4 or 8 streams that
 // share a tile's keys and are joined at its end; K and V of a stream's next four keys are on their way while four are worked on.
 // -------------------------------------------------------------------------------------------------
 constexpr int kKeysAny = 32, kThreadsAny = 128, kPerSmAny = 3, kFixedAny = 3, kSplitAny = 1;
@@ -415,7 +416,8 @@ static int64_t chunk_rows(const splat_paged_args& a) {
     const int64_t n = a.max_q_len < a.tokens ? a.max_q_len : a.tokens;
     return (n / a.stride + (n % a.stride != 0)) * (a.heads / a.kv_heads);
 }
-// Rows of a tile.  us, fp32 B32 kv 4096 H32/8 d128, one token (4 rows): 8 331, 4 see DESIGN; more than the rows there are cost what rows do
+// Rows of a tile: rows that are not there cost as much as others.  us, fp32, 32 requests of 4096 tokens, one token each, d128: 32 / 8 heads (4 rows)
+// with 8 rows 331, with 4 257; 16 / 16 heads (1 row) with 8 rows 331, with 2 237
 static int rows_any(const splat_paged_args& a) {
     const int64_t most = chunk_rows(a);
     return most <= 2 ? 2 : most <= 4 ? 4 : 8;
@@ -563,7 +565,7 @@ extern "C" int32_t splat_paged_attention(const splat_paged_args* args, void* str
         // second waits for the joining of the first
         if (chunk_rows(a) > kFewRows) {
             // One kernel for all of them where, as a rule, all bring as many, or where those of few rows are so few that a launch of their own
-            // costs more than tiles that are mostly empty (8 requests, 2 of them with chunks, 8 heads: 69 us with two launches, 46 with one)
+            // costs more than tiles that are mostly empty (8 requests, 2 of them with chunks, 8 heads: the second kernel and its joining took 12 us)
             const bool alike = a.tokens == a.requests * a.max_q_len || a.requests * a.kv_heads <= chunk_ctas(sms) / 2;
             p.rows_from = alike ? 0 : kFewRows + 1;
             const int32_t rc = attend_chunk(a, p, sms, a.workspace, st);

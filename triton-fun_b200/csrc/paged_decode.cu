@@ -8,11 +8,13 @@
 //     own running maximum, sum and output.  Nothing in the loop is shared between them; at a tile's end they are joined in shared memory.
 //   * A fifth warp walks ahead over the schedule, through the ends of tiles, and fills a ring of eight chunks, so that copies are
 //     under way while tiles are joined and begun: 128 KB on an SM with its two CTAs, where 45 KB would cover the latency at HBM speed.  It also
-//     fetches the tiles' rows of q and describes them to the others.  (Every warp filling its own ring of three, tile by tile: 64 ragged
-//     requests, see paged_schedule.cuh, 95 us.)
+//     fetches the tiles' rows of q and describes them to the others.  Four chunks at a time, one for each of the others: chunk by chunk it is
+//     the bottleneck.  us, 64 ragged requests (see paged_schedule.cuh): every warp filling a ring of three of its own, tile by tile 95; a copying
+//     warp, chunk by chunk 117, four at a time 85 (5.2 TB/s, 0.80 of the measured copy rate).
 //   * Chunks come by tiled copies (TMA) of 64 columns x 8 to 32 rows of a page, issued by as many lanes at once; a page's rows of one
 //     residue class are a box of a 5-D map (columns, residues, rows of a class, heads, pages).  That asks for pages of whole classes with
-//     a multiple of 8 rows; other pages and strides come by cp.async, 16 bytes each.  Pages are looked up for 32 boxes or keys at once.
+//     a multiple of 8 rows; other pages and strides come by cp.async, 16 bytes each
+//     (32 requests of 4096 tokens, pages of 7 rows: 2.5 TB/s).  Pages are looked up for 32 boxes or keys at once.
 //   * Rows behind the request's last token, and of pages that are not there, are masked in S, and their rows of V are set to
 //     zero in the ring, whatever they held.
 // How the work is divided over CTAs: paged_schedule.cuh.
