@@ -136,6 +136,8 @@ def attention_args():
     (dict(taps=-1), "taps must be at least 0", ValueError),
     (dict(stride=0), "stride must be at least 1", ValueError),
     (dict(softcap=-1.0), "softcap must not be negative", ValueError),
+    (dict(softcap=1e-40), "too small for the scale", ValueError),
+    (dict(softcap=1e-30, scale=1e10), "too small for the scale", ValueError),
     (dict(scale=float("nan")), "scale must be finite", ValueError),
     (dict(scale=1e300), "scale must be finite", ValueError),
     (dict(slopes=torch.zeros(2)), "an entry for each head", ValueError),
@@ -149,6 +151,21 @@ def attention_args():
 ])
 def test_attention_refusals(change, words, error):
     refused(r_paged.rpaged_attention_launcher, attention_args(), change, words, error)
+
+
+def test_c_entry_points_refuse_bad_arguments():
+    """Statuses of the C ABI for calls that launch nothing: null pointers, sizes that do not agree."""
+    import ctypes
+    import splat_native as n
+    lib, none = n._lib, None
+    assert lib.splat_paged_attention(none, none) == -1 and lib.splat_paged_attention_workspace(none) == 0
+    sections, rows = (ctypes.c_int64 * 2)(3, 4), (ctypes.c_int64 * 10)()
+    assert lib.splat_rotary(none, 1, none, 0, 0, 0, 0, none, 0, none, 0, 0, 0, 1, 1, 8, 0, none, 1, 0, none) == -1
+    assert lib.splat_rotary(rows, 1, none, 0, 0, 0, 0, none, 0, none, 0, 0, 0, 1, 1, 8, 7, none, 1, 0, none) == -2      # dtype
+    assert lib.splat_rotary(rows, 1, none, 0, 0, 0, 0, none, 5, sections, 2, 0, 0, 1, 1, 8, 0, none, 1, 0, none) == -1  # half > d / 2
+    assert lib.splat_rotary(rows, 1, none, 0, 0, 0, 0, none, 0, none, 0, 0, 0, 1, 1, 8, 0, none, 1, 0, none) == 0       # no heads: nothing to do
+    assert lib.splat_paged_tables(none, none, none, 0, none, 1, none, 16, 0, 0, 0, none, none, none, none, none, none, none) == -1
+    assert lib.splat_paged_tables(none, none, none, 0, none, 1, none, 16, 20000, 0, 0, none, none, none, none, none, none, none) == -6
 
 
 def test_module_refuses_the_cpu():

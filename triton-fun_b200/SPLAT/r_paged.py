@@ -13,7 +13,8 @@ A cache is two tensors (pages, K/V heads, page size, head size), at any strides 
 request b is row ``j % page_size`` of page ``block_table[b, j // page_size]``.  Entries of the block table outside
 ``[0, pages)`` are pages that are not there: nothing is written to them and their keys are not attended to.
 
-The launchers work with lengths that are on the device only, read nothing back, and can be captured in a CUDA graph.
+The launchers work with lengths that are on the device only, read nothing back, and can be captured in a CUDA graph.  They
+have no gradients.
 ``PagedAttention`` keeps the buffers that they need.
 """
 from __future__ import annotations

@@ -3,6 +3,7 @@
 // For query position i of head h, over the keys j = i - k stride >= 0 with k < taps:
 //     x_j = c tanh(scale q.k_j / c) or scale q.k_j;   s_j = x_j - slope_h (i - j);   o = sum_j e^(s_j - m) v_j / sum_j e^(s_j - m)
 // with m the running maximum; scores, sums and outputs are held in fp32, in powers of two.  How the work is divided: paged_schedule.cuh.
+#include <cmath>
 #include <initializer_list>
 #include <type_traits>
 
@@ -451,7 +452,8 @@ static int32_t launch_any(const splat_paged_args& a, Problem p, int ctas, cudaSt
 static int32_t check_args(const splat_paged_args& a) {
     if (a.dtype != SPLAT_F32 && a.dtype != SPLAT_F16 && a.dtype != SPLAT_BF16) return SPLAT_ERR_UNSUPPORTED_DTYPE;
     if (a.tokens < 0 || a.requests < 0 || a.pages < 0 || a.page < 1 || a.heads < 1 || a.kv_heads < 1 || a.d < 1 || a.taps < 0 || a.stride < 1 ||
-        a.table_width < 0 || a.table_stride < a.table_width || a.heads % a.kv_heads != 0 || !(a.softcap >= 0.f))
+        a.table_width < 0 || a.table_stride < a.table_width || a.heads % a.kv_heads != 0 || !(a.softcap >= 0.f) ||
+        (a.softcap > 0.f && !std::isfinite(a.scale / a.softcap)))
         return SPLAT_ERR_BAD_ARG;
     if (a.requests > SPLAT_PAGED_MAX_REQUESTS || a.d > 256 || a.pages > INT32_MAX || a.page > kMaxLen || a.table_width > kMaxLen ||
         a.table_width * a.page > kMaxLen || a.heads > 65535 || a.tokens >= kMaxLen / a.heads)

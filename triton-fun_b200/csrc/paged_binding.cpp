@@ -469,6 +469,7 @@ PyObject* paged_attention(PyObject* const* a, Py_ssize_t n) {
     x.stride = integer(a[10], "stride", 1);
     x.softcap = number(a[11], "softcap");
     if (x.softcap < 0.f) refuse("softcap must not be negative");
+    if (x.softcap > 0.f && !std::isfinite(x.scale / x.softcap)) refuse("softcap is too small for the scale");
     if (given(a[12])) {
         slopes = tensor(a[12], "slopes", 1);
         of_type(slopes, at::kFloat, "float32");
