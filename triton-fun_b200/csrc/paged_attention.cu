@@ -27,7 +27,7 @@ __device__ __forceinline__ float score_of(const Problem& p, float dot) {
 // their way 519.  A block's 4 warps are 4 or 8 streams that
 // share a tile's keys and are joined at its end; K and V of a stream's next four keys are on their way while four are worked on.
 // -------------------------------------------------------------------------------------------------
-constexpr int kKeysAny = 32, kThreadsAny = 128, kPerSmAny = 3, kFixedAny = 3, kSplitAny = 1;
+constexpr int kKeysAny = 32, kThreadsAny = 128, kPerSmAny = 3, kFixedAny = 3, kSplitAny = 1, kWholeAny = 3;
 
 template <int kLanes, int R> __device__ __forceinline__ float reduce_rows(float (&v)[R], int lane) {
 #pragma unroll
@@ -437,6 +437,7 @@ static int32_t launch_any(const splat_paged_args& a, Problem p, int ctas, cudaSt
                       fits(a.v_cache, {a.v_page, a.v_head, a.v_row});
     const int rows = rows_any(a), d_pad = d_pad_any(a.d);
     Layout(ctas, rows, d_pad).place(p, a.workspace);
+    p.whole_tiles = few_steps(a, rows, kKeysAny, kWholeAny, ctas);
     auto of = [&](auto lanes, auto cols) {
         constexpr int kLanes = decltype(lanes)::value, kC = decltype(cols)::value;
         return rows == 8 ? paged_rows_kernel<T, kLanes, kC, 8> : rows == 4 ? paged_rows_kernel<T, kLanes, kC, 4> : paged_rows_kernel<T, kLanes, kC, 2>;
@@ -446,7 +447,7 @@ static int32_t launch_any(const splat_paged_args& a, Problem p, int ctas, cudaSt
                 : d_pad == 128 ? of(integral_constant<int, 32>(), integral_constant<int, kCols>())
                                : of(integral_constant<int, 32>(), integral_constant<int, 2 * kCols>());
     const int32_t rc = launch_kernel(kern, dim3((unsigned)ctas), dim3(kThreadsAny), 0, st, p, wide);
-    return rc != SPLAT_OK ? rc : join_parts(p, ctas, rows, d_pad, a.dtype, st);
+    return rc != SPLAT_OK || p.whole_tiles ? rc : join_parts(p, ctas, rows, d_pad, a.dtype, st);
 }
 
 static int32_t check_args(const splat_paged_args& a) {

@@ -38,6 +38,7 @@ using sm::pack2;
 constexpr int kRows = 128, kKeys = 128, kThreads = 192, kTmaWarp = 4, kMmaWarp = 5;
 constexpr int kFixed = 2;                       // what a tile costs beside its steps, in steps
 constexpr int kSplit = 8;                       // what dividing one costs
+constexpr int kWhole = 4;                       // tiles of up to so many steps are not divided where none has more
 constexpr int kTmemCols = 256, kPerSm = 2;
 constexpr float kLazy = 8.f;                    // log2: the maximum is raised when it has grown by more
 enum : int { kErrPiece = 91, kErrPieceFree, kErrQ, kErrQFree, kErrOFree, kErrKFull, kErrKFree, kErrVFull, kErrVFree, kErrVLanded, kErrS, kErrSFree, kErrP, kErrPv, kErrO };
@@ -660,6 +661,7 @@ int32_t attend_chunk(const splat_paged_args& a, Problem p, int sms, void* worksp
         !cache_map(&maps.v, a, a.v_cache, a.v_page, a.v_head, a.v_row, box))
         return SPLAT_ERR_UNSUPPORTED_SHAPE;
     paged::Layout(ctas, kRows, d_pad).place(p, workspace);
+    p.whole_tiles = few_steps(a, kRows, kKeys, kWhole, ctas);
     const FastDiv class_page((uint32_t)(a.page / a.stride));
     const bool q_wide = aligned16(a.q) && a.q_row % 8 == 0 && a.q_head % 8 == 0;
     const int64_t group = a.heads / a.kv_heads;
@@ -670,7 +672,7 @@ int32_t attend_chunk(const splat_paged_args& a, Problem p, int sms, void* worksp
                            : launch<T, 128>(p, ctas, maps, box, class_page, q_wide, q_tma, st);
     };
     const int32_t rc = a.dtype == SPLAT_BF16 ? run(__nv_bfloat16()) : run(__half());
-    return rc != SPLAT_OK ? rc : join_parts(p, ctas, kRows, d_pad, a.dtype, st);
+    return rc != SPLAT_OK || p.whole_tiles ? rc : join_parts(p, ctas, kRows, d_pad, a.dtype, st);
 }
 
 }  // namespace paged

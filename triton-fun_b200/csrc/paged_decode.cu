@@ -38,6 +38,7 @@ using sm::pack2;
 constexpr int kWarps = 4, kThreads = 160, kCopyWarp = 4, kRows = 16, kSlots = 8;
 constexpr int kFixed = 2;            // what a tile costs beside its steps, in steps (us, the two cases: 0 155 / 140, 1 91 / 93, 2 85.6 / 80.3, 4 86.4 / 81.7)
 constexpr int kSplit = 1;            // what dividing one costs
+constexpr int kWhole = 5;            // tiles of up to so many steps are not divided where none has more
 constexpr float kLazy = 8.f;         // log2: the maximum is raised when it has grown by more
 
 // codes of the status word
@@ -521,6 +522,7 @@ int32_t attend_decode(const splat_paged_args& a, Problem p, int sms, void* works
     const int d_pad = a.d <= 64 ? 64 : 128;
     paged::Layout(decode_ctas(sms), kRows, d_pad).place(p, workspace);
     const bool q_wide = aligned16(a.q) && a.q_row % 8 == 0 && a.q_head % 8 == 0;
+    p.whole_tiles = few_steps(a, kRows, d_pad == 64 ? Shape<64>::kKeys : Shape<128>::kKeys, kWhole, decode_ctas(sms));
     const int box = box_rows(a, d_pad == 128 ? 16 : 32);
     Maps maps;
     const bool tma = a.status_word != nullptr && box >= 8 && cache_map(&maps.k, a, a.k_cache, a.k_page, a.k_head, a.k_row, box) &&
@@ -532,7 +534,7 @@ int32_t attend_decode(const splat_paged_args& a, Problem p, int sms, void* works
                            : launch<T, 128>(p, sms, tma ? &maps : nullptr, box, class_page, q_wide, st);
     };
     const int32_t rc = a.dtype == SPLAT_BF16 ? run(__nv_bfloat16()) : run(__half());
-    return rc != SPLAT_OK ? rc : join_parts(p, decode_ctas(sms), kRows, d_pad, a.dtype, st);
+    return rc != SPLAT_OK || p.whole_tiles ? rc : join_parts(p, decode_ctas(sms), kRows, d_pad, a.dtype, st);
 }
 
 }  // namespace paged

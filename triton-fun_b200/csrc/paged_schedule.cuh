@@ -48,6 +48,7 @@ struct Problem {
     int table_rows;                    // tokens that the table has room for
     int taps;
     FastDiv group, stride, page_div;   // query heads per K/V head
+    bool whole_tiles;                  // hand out tiles whole, whatever the lengths (and join nothing)
     int rows_from, rows_to;            // requests with so many rows in a class are this kernel's
     float scale_log2, softcap, cap_inv;    // x = qk * scale_log2, or softcap_log2 * tanh(qk * cap_inv)
     float2 cap_poly[7];                // softcap_log2 * tanh(y) / y in powers of y^2, twice each (see paged_rows.cuh)
@@ -195,7 +196,7 @@ struct Walk {
             most = max(most, sh.warp_most[w]);
         }
         const int64_t cost_share = divide(cost_all + gridDim.x - 1, gridDim.x), tiles_share = divide(tiles_all + gridDim.x - 1, gridDim.x);
-        by_tile = tiles_share * most <= cost_share + kSplit;
+        by_tile = p.whole_tiles || tiles_share * most <= cost_share + kSplit;
         sh.before[threadIdx.x + 1] = by_tile ? tiles_sum : cost_sum;
         if (threadIdx.x == 0) sh.before[0] = 0;
         __syncthreads();
@@ -305,6 +306,17 @@ __device__ __forceinline__ int64_t cache_row(const Problem& p, const int32_t* ta
     const int page = __ldg(table + i);
     if (page < 0 || page >= p.pages) return -1;
     return page * page_stride + ((int)j - i * (int)p.page_div.d) * row_stride;
+}
+
+// Whether tiles are so few (two for each CTA at most) and have so few steps, whatever the lengths, that none is worth dividing: by what the table has
+// room for, or by the window.  The joining launch, 3 us of the smallest calls' 10, is left out then.  (More tiles are better divided: 128 requests of
+// 1 to 256 tokens, 8 heads, 24.4 us divided, 31.5 whole.)
+inline bool few_steps(const splat_paged_args& a, int rows, int keys, int most, int ctas) {
+    const int64_t stride = a.stride < kMaxLen ? a.stride : kMaxLen, room = (a.table_width * a.page + stride - 1) / stride;
+    const int64_t window = a.taps > 0 && a.taps < kMaxLen ? a.taps + rows : kMaxLen;       // (a tile's rows are of so many tokens at most)
+    const int64_t classes = a.requests * stride < a.tokens ? a.requests * stride : a.tokens;
+    const int64_t tiles = (a.tokens * (a.heads / a.kv_heads) / rows + classes) * a.kv_heads;
+    return tiles <= 2 * ctas && (room < window ? room : window) <= (int64_t)(most - 1) * keys;     // (one more step where they do not begin with one)
 }
 
 // What a kernel of this kind needs of workspace.
