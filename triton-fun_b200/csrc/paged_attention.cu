@@ -73,7 +73,7 @@ __device__ __forceinline__ void load_cols(const T* row, int col0, int d, bool wi
 template <typename T, int kLanes, int kCols, int R>
 __global__ void __launch_bounds__(kThreadsAny, kCols == 4 ? kPerSmAny : 2) paged_rows_kernel(const Problem p, const bool wide) {
     constexpr int kStreams = kThreadsAny / kLanes, kD = kLanes * kCols, kBatch = kCols == 4 ? 4 : 2;       // keys of a stream's round
-    using Part = Walk<R, kKeysAny, kThreadsAny, kFixedAny, kSplitAny, false>;
+    using Part = Walk<R, kKeysAny, kThreadsAny, kFixedAny, kSplitAny, true>;
     __shared__ union Shared {
         WalkShared<kThreadsAny> walk;
         struct { float m[kStreams][R], l[kStreams][R], o[kStreams][R][kD]; } join;
