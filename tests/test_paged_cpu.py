@@ -203,3 +203,23 @@ def test_oracle_rotary_turns_back():
         y = po.rotary(x, pos, freq, (2, 3), interleaved)
         assert torch.allclose(po.rotary(y, pos, freq, (2, 3), interleaved, inverse=True), x)
         assert torch.equal(y[..., 10:], x[..., 10:])
+
+
+@pytest.mark.parametrize("row, length, freed", [([4, 2, -1, -1, -1, -1, -1], 17, [4, 2]), ([4, -1, 2, -1, -1, -1, -1], 17, [4, 2]),
+                                                ([-1] * 7, 28, []), ([0, 1, 2, 3, 4, -1, -1], 28, [0, 1, 2, 3, 4]), ([-1] * 7, 0, [])])
+def test_release_of_a_request_that_was_short_of_pages(row, length, freed):
+    """Pages that were missing are no pages to hand out again, and a request that is released twice has none to give."""
+    m = r_paged.PagedAttention.__new__(r_paged.PagedAttention)
+    torch.nn.Module.__init__(m)
+    m.device, m.page_size = torch.device("cpu"), 4
+    m.block_table = torch.tensor([[-1] * 7, row], dtype=torch.int32)
+    held = [p for p in range(5) if p not in freed]
+    m.free_pages = torch.full((5,), 77, dtype=torch.int32)
+    m.free_span = torch.tensor([8, 8 + len(held)])
+    for i, p in enumerate(held):
+        m.free_pages[(8 + i) % 5] = p
+    for _ in range(2):
+        m.release(1, length)
+        assert m.free_span.tolist() == [8, 13]
+        assert [int(m.free_pages[i % 5]) for i in range(8, 13)] == held + freed
+        assert m.block_table.eq(-1).all()
