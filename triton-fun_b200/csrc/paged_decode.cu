@@ -10,11 +10,14 @@
 //     under way while tiles are joined and begun: 128 KB on an SM with its two CTAs, where 45 KB would cover the latency at HBM speed.  It also
 //     fetches the tiles' rows of q and describes them to the others.  Four chunks at a time, one for each of the others: chunk by chunk it is
 //     the bottleneck.  us, 64 ragged requests (see paged_schedule.cuh): every warp filling a ring of three of its own, tile by tile 95; a copying
-//     warp, chunk by chunk 117, four at a time 85 (5.2 TB/s, 0.80 of the measured copy rate).
+//     warp, chunk by chunk 117, four at a time 85.
 //   * Chunks come by tiled copies (TMA) of 64 columns x 8 to 32 rows of a page, issued by as many lanes at once; a page's rows of one
 //     residue class are a box of a 5-D map (columns, residues, rows of a class, heads, pages).  That asks for pages of whole classes with
 //     a multiple of 8 rows; other pages and strides come by cp.async, 16 bytes each
 //     (32 requests of 4096 tokens, pages of 7 rows: 2.5 TB/s).  Pages are looked up for 32 boxes or keys at once.
+//   * A tile seldom has all 16 rows, and its end is spent on those that it has: with all of them joined, and written where a tile is divided,
+//     the same 85 (81: 5.5 TB/s, 0.84 of the measured copy rate), 96 windows of up to 1024 keys with 16 / 16 heads 80 (73), 96 requests of 128
+//     tokens 35 (28).
 //   * Rows behind the request's last token, and of pages that are not there, are masked in S, and their rows of V are set to
 //     zero in the ring, whatever they held.
 // How the work is divided over CTAs: paged_schedule.cuh.
@@ -36,7 +39,7 @@ using sm::ex2;
 using sm::pack2;
 
 constexpr int kWarps = 4, kThreads = 160, kCopyWarp = 4, kRows = 16, kSlots = 8;
-constexpr int kFixed = 2;            // what a tile costs beside its steps, in steps (us, the two cases: 0 155 / 140, 1 91 / 93, 2 85.6 / 80.3, 4 86.4 / 81.7)
+constexpr int kFixed = 2;            // what a tile costs beside its steps, in steps (us, 64 ragged requests of one token / of four: 0 124 / 189, 1 81.5 / 111, 2 81.3 / 86.5)
 constexpr int kSplit = 1;            // what dividing one costs
 constexpr int kWhole = 5;            // tiles of up to so many steps are not divided where none has more
 constexpr float kLazy = 8.f;         // log2: the maximum is raised when it has grown by more
@@ -449,7 +452,8 @@ paged_decode_kernel(const __grid_constant__ Maps maps, const __grid_constant__ P
                 if (lane == 0) tc::mbar_arrive(&ctrl->empty[slot]);
             }
             n_chunk += x.chunks;
-            // The warps' parts, joined
+            // The warps' parts, joined.  Rows that the tile does not have (heads without a group: 15 of 16) are left out
+            const int rows_here = x.count * g - x.base;
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
                 sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 1);
@@ -460,15 +464,20 @@ paged_decode_kernel(const __grid_constant__ Maps maps, const __grid_constant__ P
                 }
             }
 #pragma unroll
-            for (int n = 0; n < D / 8; ++n)
+            for (int r = 0; r < 2; ++r)
+                if (quad + 8 * r < rows_here)
 #pragma unroll
-                for (int r = 0; r < 2; ++r)
-                    *reinterpret_cast<float2*>(parts + (warp * kRows + quad + 8 * r) * D + n * 8 + in_quad * 2) = make_float2(o[n][2 * r], o[n][2 * r + 1]);
+                    for (int n = 0; n < D / 8; ++n)
+                        *reinterpret_cast<float2*>(parts + (warp * kRows + quad + 8 * r) * D + n * 8 + in_quad * 2) = make_float2(o[n][2 * r], o[n][2 * r + 1]);
             if (any_of_the_four(!ok)) break;
             constexpr int kLanes = D / 4;                      // threads to a row, four columns each
 #pragma unroll
             for (int r0 = 0; r0 < kRows; r0 += kWarps * 32 / kLanes) {
                 const int r = r0 + threadIdx.x / kLanes, col = (threadIdx.x % kLanes) * 4, m = token_of(r);
+                if (r >= rows_here) {
+                    if (!x.whole && col == 0) p.part_rows[(int64_t)x.part * kRows + r] = make_float4(-INFINITY, 0.f, __int_as_float(-1), 0.f);
+                    continue;
+                }
                 float most = -INFINITY, all = 0.f;
                 float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
