@@ -543,3 +543,12 @@ def test_captured_serving_step():
             want, _, tol, _ = po.attention(q, m.k_cache[0], m.v_cache[0], m.block_table, m.kv_lens, m.q_start, scale=d ** -0.5)
             assert bool(((m.output.double() - want).abs() <= tol).all())
     assert m.kv_lens.tolist() == [40] * B and m.missing_pages() == 0
+
+
+def test_log_sums_in_another_operands_place_are_refused():
+    q, cache = torch.zeros(2, 4, 4, device="cuda"), torch.zeros(3, 4, 2, 4, device="cuda")
+    table, lens = torch.zeros(2, 1, dtype=torch.int32, device="cuda"), torch.ones(2, dtype=torch.int32, device="cuda")
+    out, other = torch.zeros_like(q), torch.zeros_like(cache)
+    for lse in (q.view(-1)[:8].view(2, 4), out.view(-1)[:8].view(2, 4), cache.view(-1)[:8].view(2, 4)):
+        with pytest.raises(ValueError, match="share memory"):
+            r_paged.rpaged_attention_launcher(q, cache, other, table, lens, out, lse=lse)

@@ -223,3 +223,20 @@ def test_release_of_a_request_that_was_short_of_pages(row, length, freed):
         assert m.free_span.tolist() == [8, 13]
         assert [int(m.free_pages[i % 5]) for i in range(8, 13)] == held + freed
         assert m.block_table.eq(-1).all()
+
+
+def test_outputs_are_the_operands_themselves_or_elsewhere():
+    """In place means at the same strides: a row written before it is read as another one would be a wrong answer."""
+    x = torch.zeros(2, 4, 4, 16)
+    turned = x.transpose(1, 2)
+    for kw, words in [(dict(q=x, k=None, q_out=turned), "q_out must be q itself"), (dict(q=x, k=x.clone(), q_out=x, k_out=x), "share memory"),
+                      (dict(q=x.clone(), k=x, q_out=x), "share memory"), (dict(q=x, k=turned, k_out=x), "share memory"),
+                      (dict(q=x, k=None, q_out=x), "CUDA devices only")]:
+        refused(r_rotary.rrotary_launcher, dict(positions=i32(4), inv_freq=torch.zeros(8), **kw), {}, words)
+    kw = append_args()
+    for change, words in [(dict(q_out=kw["q"]), "CUDA devices only"), (dict(q_out=kw["k"].expand(5, 2, 16), q=kw["v"]), "share memory"),
+                          (dict(q=kw["q"][:, :2], q_out=kw["v"]), "share memory"),
+                          (dict(q=kw["q"].view(4, 5, 16).transpose(0, 1), q_out=kw["q"]), "q_out must be q itself"),
+                          (dict(q_out=kw["k_cache"].view(6, 8, 16)[:5, :4]), "share memory"),
+                          (dict(q=kw["k_cache"].view(6, 8, 16)[:5, :4]), "share memory")]:
+        refused(r_paged.rpaged_append_launcher, kw, change, words)

@@ -114,6 +114,12 @@ void distinct(const Operand& x, const Operand& y) {
     if (x->numel() > 0 && y->numel() > 0 && x->const_data_ptr() == y->const_data_ptr())
         refuse(std::string(x.name) + " and " + y.name + " must not share memory");
 }
+// the same, unless x is y itself
+void itself_or_distinct(const Operand& x, const Operand& y) {
+    if (x->numel() == 0 || x->const_data_ptr() != y->const_data_ptr()) return;
+    for (int64_t i = 0; i < x->dim(); ++i)
+        if (x->size(i) > 1 && x->stride(i) != y->stride(i)) refuse(std::string(x.name) + " must be " + y.name + " itself or not share memory with it");
+}
 void check(int32_t rc, const char* what) {
     if (rc != 0)
         throw Refused{PyExc_RuntimeError, std::string(what) + ": splat status " + std::to_string(rc) + " (" + g_status_string(rc) + ")"};
@@ -248,7 +254,10 @@ void rotate(Operand (&in)[2], Operand (&out)[2], at::Tensor (&made)[2], const Op
         if (out[i]->sizes() != in[i]->sizes()) refuse(std::string(names[i]) + " must have the shape of its operand");
         rows_contiguous(out[i]);
         no_overlap(out[i]);
+        itself_or_distinct(out[i], in[i]);
+        if (count == 2) distinct(out[i], in[1 - i]);
     }
+    if (out[0].t != nullptr && out[1].t != nullptr) distinct(out[0], out[1]);
     const int dev = device_of({in[0], in[1], t.positions, t.inv_freq, out[0], out[1]});
     c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(dev));
     splat_rows rows[2] = {};
@@ -403,6 +412,9 @@ PyObject* paged_append(PyObject* const* a, Py_ssize_t n) {
         rows_contiguous(q);
         rows_contiguous(q_out);
         no_overlap(q_out);
+        itself_or_distinct(q_out, q);
+        for (const Operand* x : {&k, &v, &kc, &vc}) distinct(q_out, *x);
+        for (const Operand* x : {&kc, &vc}) distinct(*x, q);
     }
     Turn t;
     const bool turned = given(a[7]);
@@ -485,7 +497,11 @@ PyObject* paged_attention(PyObject* const* a, Py_ssize_t n) {
     if (c.pages > INT32_MAX || table->size(1) > (1 << 30) / c.page || T >= (1 << 30) / H)
         refuse("pages, tokens of a request or tokens times heads beyond what the kernels count (2^31, 2^30)");
     const int dev = device_of({q, kc, vc, table, kv, out, start, slopes, lse});
-    for (const Operand* y : {&q, &kc, &vc}) distinct(out, *y);
+    for (const Operand* y : {&q, &kc, &vc}) {
+        distinct(out, *y);
+        if (lse.t != nullptr) distinct(lse, *y);
+    }
+    if (lse.t != nullptr) distinct(lse, out);
     if (T == 0 || B == 0) Py_RETURN_NONE;
     c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(dev));
     if (x.dtype != SPLAT_F32) {
