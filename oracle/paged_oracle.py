@@ -1,6 +1,6 @@
 """64-bit restatement of the paged cache's operators, of the rotary positions, and of the error that rounding allows.
 
-Checker only.  Everything is written from the formulas, request by request and head by head, and runs on any device.
+An oracle, no part of the product.  Everything is written from the formulas, request by request and head by head, and runs on any device.
 """
 from __future__ import annotations
 
