@@ -414,6 +414,13 @@ typedef struct {
 int64_t splat_paged_attention_workspace(const splat_paged_args* args);
 int32_t splat_paged_attention(const splat_paged_args* args, void* stream);
 
+/* Test helper: the launch that joins divided tiles alone, over a workspace that the caller has filled as `ctas` CTAs with tiles of `rows` rows
+ * leave it, with D = 64, 128 or 256 >= d: int64 begins[ctas] (the step that the tile begins with in whose middle CTA c begins, or -1), from the next multiple
+ * of 16 bytes float part_rows[2 ctas][rows][4] (maximum in the log2 domain, sum, and the bits of token and head) and part_o[2 ctas][rows][D].  Part 2 c is of
+ * the tile that CTA c begins in the middle of, 2 c + 1 of its last.  Rows of tokens or heads that the call does not have stay
+ * unwritten, and so does everything while *status_word is not 0. */
+int32_t splat_selftest_paged_join(const splat_paged_args* args, int32_t ctas, int32_t rows, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

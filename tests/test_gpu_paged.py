@@ -1,4 +1,5 @@
 """GPU: block tables, the paged cache and attention over it, against 64 bits."""
+import math
 import random
 
 import pytest
@@ -552,3 +553,63 @@ def test_log_sums_in_another_operands_place_are_refused():
     for lse in (q.view(-1)[:8].view(2, 4), out.view(-1)[:8].view(2, 4), cache.view(-1)[:8].view(2, 4)):
         with pytest.raises(ValueError, match="share memory"):
             r_paged.rpaged_attention_launcher(q, cache, other, table, lens, out, lse=lse)
+
+
+def joined(rows_of, begins, rows=4, d=8, tokens=3, heads=2, status=0):
+    """splat_selftest_paged_join over the parts (part, row) -> (maximum, sum, token, head, value), in an output with room around it."""
+    import ctypes
+    import splat_native as n
+
+    class Args(ctypes.Structure):
+        _fields_ = [(f, ctypes.c_void_p) for f in ("q", "k_cache", "v_cache", "o", "lse")] + \
+                   [(f, ctypes.c_int64) for f in ("q_row", "q_head", "o_row", "o_head", "k_page", "k_head", "k_row", "v_page", "v_head", "v_row")] + \
+                   [("block_table", ctypes.c_void_p), ("table_stride", ctypes.c_int64), ("table_width", ctypes.c_int64)] + \
+                   [(f, ctypes.c_void_p) for f in ("kv_lens", "q_start", "slopes")] + \
+                   [(f, ctypes.c_int64) for f in ("tokens", "requests", "pages", "page", "heads", "kv_heads", "d", "taps", "stride", "max_q_len")] + \
+                   [("scale", ctypes.c_float), ("softcap", ctypes.c_float), ("dtype", ctypes.c_int32), ("status_word", ctypes.c_void_p),
+                    ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_int64)]
+
+    ctas, at = len(begins), -(-len(begins) * 8 // 16) * 16
+    work = torch.zeros(at + 2 * ctas * rows * 16 + 2 * ctas * rows * 64 * 4, dtype=torch.uint8, device="cuda")
+    work[:ctas * 8].view(torch.int64).copy_(ints(begins, torch.int64))
+    ends = work[at:at + 2 * ctas * rows * 16].view(torch.float32).view(2 * ctas, rows, 4)
+    sums = work[at + 2 * ctas * rows * 16:].view(torch.float32).view(2 * ctas, rows, 64)
+    ends[:, :, 2:].view(torch.int32).fill_(-1)
+    for (part, row), (top, total, token, head, value) in rows_of.items():
+        ends[part, row, :2] = torch.tensor([top, total], device="cuda")
+        ends[part, row, 2:].view(torch.int32).copy_(ints([token, head]))
+        sums[part, row, :d] = value
+    around = torch.full((50, heads, d), 7.0, device="cuda")
+    lse = torch.full((50, heads), 7.0, device="cuda")
+    word = ints([status])
+    out, out_lse = around[20:20 + tokens], lse[20:20 + tokens]
+    x = Args(o=out.data_ptr(), lse=out_lse.data_ptr(), o_row=heads * d, o_head=d, tokens=tokens, requests=1, pages=1, page=16, heads=heads,
+             kv_heads=1, d=d, stride=1, status_word=word.data_ptr(), workspace=work.data_ptr(), workspace_bytes=work.numel())
+    assert n._lib.splat_selftest_paged_join(ctypes.byref(x), ctas, rows, torch.cuda.current_stream().cuda_stream) == 0
+    torch.cuda.synchronize()
+    rest = torch.ones(50, dtype=torch.bool)
+    rest[20:20 + tokens] = False
+    assert bool((around[rest] == 7).all()) and bool((lse[rest] == 7).all())
+    return out.cpu(), out_lse.cpu()
+
+
+def test_joining_of_parts_that_a_kernel_never_wrote():
+    """A kernel that gives up has announced parts that it does not write: the workspace holds anything.  Rows that the call does not have
+    are not written, and none is while the status word is set."""
+    good = {(1, 0): (0.0, 1.0, 0, 1, 2.0), (2, 0): (1.0, 1.0, 0, 1, 8.0)}
+    # (0 + 2^0 2 + 2^1 8) / (2^0 + 2^1), and its log-sum-exp
+    out, lse = joined(good, [-1, 0, -1])
+    assert bool(((out[0, 1] - 6.0).abs() < 1e-5).all()) and abs(float(lse[0, 1]) - math.log(3)) < 1e-6 and bool((out[0, 0] == 7).all())
+    for token, head in ((3, 0), (5, 1), (-1, 0), (-17, 0), (1, 2), (1, -1), (0, 9), (29, 0)):
+        bad = {**good, (1, 1): (0.0, 1.0, token, head, 3.0), (2, 1): (0.0, 1.0, token, head, 3.0)}
+        for begins in ([-1, 0, -1], [-1, 0, -1, -1, -1]):  # a warp to a row, and four
+            out, lse = joined(bad, begins)
+            assert bool(((out[0, 1] - 6.0).abs() < 1e-5).all())
+            out[0, 1], lse[0, 1] = 7.0, 7.0
+            assert bool((out == 7).all()) and bool((lse == 7).all()), (token, head)
+    for begins in ([-1, 0, -1], [-1, 0, -1, -1, -1]):
+        out, lse = joined(good, begins, status=81)
+        assert bool((out == 7).all()) and bool((lse == 7).all())
+    # tiles of 32 rows: a warp to a row
+    out, lse = joined({**good, (1, 30): (0.0, 1.0, 29, 0, 3.0), (2, 31): (0.0, 1.0, 3, 0, 3.0)}, [-1, 0, -1], rows=32)
+    assert bool(((out[0, 1] - 6.0).abs() < 1e-5).all()) and bool((out[1:] == 7).all())

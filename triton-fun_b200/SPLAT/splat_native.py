@@ -79,6 +79,7 @@ SIGNATURES = {
                      _vp, _i64, _i64, _vp],
     "splat_paged_attention_workspace": [_vp],
     "splat_paged_attention": [_vp, _vp],
+    "splat_selftest_paged_join": [_vp, _i32, _i32, _vp],
 }
 for _name, _args in SIGNATURES.items():
     _fn = getattr(_lib, _name)

@@ -274,6 +274,8 @@ __global__ void __launch_bounds__(kThreadsAny, kCols == 4 ? kPerSmAny : 2) paged
 // kernel that wrote them, as a launch that is already waiting when that ends.  What it costs is round trips to memory, so a row of a small
 // tile, which may have many parts (one request of 8192 tokens: 37), has four warps that take every fourth part each, and the first parts
 // are requested before it is known what they weigh.
+// A kernel that gave up, or that was stopped by the status word, has not written all of the parts that it announced: the workspace may hold anything
+// then, an earlier call's rows among it.  So nothing leaves while the word is set, and never a row that the call does not have.
 // -------------------------------------------------------------------------------------------------
 constexpr int kThreadsJoin = 512, kWarpsJoin = kThreadsJoin / 32;
 
@@ -284,6 +286,7 @@ __global__ void __launch_bounds__(kThreadsJoin) paged_join_kernel(const Problem 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = blockIdx.x + 1, which = warp % kOfRow;
     depend_wait();
     depend_release();
+    const int32_t seen_status = p.status != nullptr ? *(const volatile int32_t*)p.status : 0;
     // One look at the CTA's neighbours: c - 1, c, c + 1, ... by lane
     const int64_t seen = c - 1 + lane < ctas ? p.begins[c - 1 + lane] : -1;
     const int64_t id = __shfl_sync(0xffffffffu, seen, 1);
@@ -311,7 +314,9 @@ __global__ void __launch_bounds__(kThreadsJoin) paged_join_kernel(const Problem 
             for (int e = 0; e < kEach; ++e)
                 x[k][e] = real && which + k * kOfRow < n ? columns(which + k * kOfRow, e) : make_float4(0.f, 0.f, 0.f, 0.f);
         float4 mine = real && lane < n ? p.part_rows[part(lane)] : make_float4(-INFINITY, 0.f, __int_as_float(-1), 0.f);
-        const int token = __float_as_int(__shfl_sync(0xffffffffu, mine.z, 0)), head = __float_as_int(__shfl_sync(0xffffffffu, mine.w, 0));
+        const int head = __float_as_int(__shfl_sync(0xffffffffu, mine.w, 0));
+        int token = __float_as_int(__shfl_sync(0xffffffffu, mine.z, 0));
+        if (token >= p.tokens || head < 0 || head >= p.kv_heads * (int)p.group.d || __shfl_sync(0xffffffffu, seen_status, 0) != 0) token = -1;
         float all = 0.f;
         float4 o[kEach];
 #pragma unroll
@@ -525,6 +530,23 @@ extern "C" int64_t splat_paged_attention_workspace(const splat_paged_args* a) {
         return chunk_rows(*a) > kFewRows && many > few ? many : few;
     }
     return Layout(sms * kPerSmAny, rows_any(*a), d_pad_any(a->d)).bytes;
+}
+
+// Where a call's parts lie, and its output: what the joining knows.
+extern "C" int32_t splat_selftest_paged_join(const splat_paged_args* args, int32_t ctas, int32_t rows, void* stream) {
+    using namespace splat;
+    using namespace splat::paged;
+    if (!args || check_args(*args) != SPLAT_OK || ctas < 1 || rows < 1 || !args->o || !args->workspace || !aligned16(args->workspace)) return SPLAT_ERR_BAD_ARG;
+    const splat_paged_args& a = *args;
+    const Layout layout(ctas, rows, d_pad_any(a.d));
+    if (a.workspace_bytes < layout.bytes) return SPLAT_ERR_SCRATCH_TOO_SMALL;
+    Problem p = {};
+    p.o = a.o; p.lse = a.lse; p.o_row = a.o_row; p.o_head = a.o_head;
+    p.tokens = (int)a.tokens; p.requests = (int)a.requests; p.kv_heads = (int)a.kv_heads; p.d = (int)a.d;
+    p.group = FastDiv((uint32_t)(a.heads / a.kv_heads));
+    p.status = a.status_word;
+    layout.place(p, a.workspace);
+    return join_parts(p, ctas, rows, d_pad_any(a.d), a.dtype, (cudaStream_t)stream);
 }
 
 extern "C" int32_t splat_paged_attention(const splat_paged_args* args, void* stream) {
