@@ -224,6 +224,30 @@ def test_what_masked_keys_hold_does_not_matter(dtype, bad):
                 assert bool(((lse[t].double() - want[1][t]).abs() <= want[3][t]).all()), (t, i)
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("kw", [dict(softcap=30.0), dict(softcap=30.0, taps=50), dict(softcap=30.0, stride=2), dict(softcap=3.0), dict()],
+                         ids=lambda kw: " ".join(f"{k}{v}" for k, v in kw.items()))
+def test_keys_that_no_query_sees_do_not_change_a_bit(dtype, d, kw):
+    """Rows of the cache behind the last token, keys in front of every window and pages that are missing."""
+    x = batch(dtype, [(200, 100), (75, 40), (330, 1)], 4, 2, d, 16)
+    x["block_table"][0, 9] = -1                            # 144 to 159
+    rows = []                                              # (page, row) that no query sees
+    for b, (kv, n) in enumerate(((200, 100), (75, 40), (330, 1))):
+        seen = {j for i in range(kv - n, kv) for j in list(range(i, -1, -kw.get("stride", 1)))[:kw.get("taps") or None]}
+        for j in range(-(-kv // 16) * 16):
+            if j not in seen and int(x["block_table"][b, j // 16]) >= 0:
+                rows.append((int(x["block_table"][b, j // 16]), j % 16))
+    pages, at = (ints(v, torch.int64) for v in zip(*rows))
+    first = None
+    for held in (float("nan"), 0.0, 300.0, -6e4, float("inf"), 0.0):
+        x["k_cache"][pages, :, at] = held
+        x["v_cache"][pages, :, at] = held if math.isfinite(held) else 1.0      # (a row that meets infinity is computed again, otherwise)
+        got = attend(x, scale=d ** -0.5, **kw)
+        first = first or got
+        assert torch.equal(got[0], first[0]) and torch.equal(got[1], first[1]), held
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_what_seen_keys_hold_matters(dtype):
     x = batch(dtype, [(40, 20)], 2, 1, 64, 16)

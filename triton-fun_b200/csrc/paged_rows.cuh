@@ -73,29 +73,38 @@ __device__ __forceinline__ float capped(const Problem& p, float dot) {
     return p.softcap - __fdividef(2.f * p.softcap, e + 1.f);
 }
 
-// The same of 128 scores in registers, where none of the warp's is beyond the cap, as is the rule (caps of 30 to 50 and scores of some 10): c
-// tanh y = c y P(y^2) on the FMA units, two at a time, instead of two more special functions for each.  P: the polynomial of degree 6 that
+// The same of 128 scores in registers: up to the cap (as is the rule: caps of 30 to 50 and scores of some 10) c tanh y = c y P(y^2) on the FMA
+// units, two at a time, instead of two more special functions for each; beyond it as above.  P: the polynomial of degree 6 that
 // agrees with tanh(sqrt z) / sqrt z at the seven Chebyshev nodes of [0, 1]; off by 5e-8 of the value.
+// Which of the two a score takes is a matter of its own size alone.  Among the 128 are keys that no row sees and columns that nothing was multiplied
+// into, with whatever memory held; they decide about the time (whether a warp looks for scores beyond the cap), never about a value.
 constexpr float kTanhPoly[7] = {0.999999949f, -0.33332828f, 0.133250761f, -0.0534516464f, 0.0202797083f, -0.00619432483f, 0.0010380251f};
 template <int N> __device__ __forceinline__ void cap_scores(const Problem& p, uint32_t (&r)[N]) {
+    const float2 inv = make_float2(p.cap_inv, p.cap_inv);
     float big = 0.f;
 #pragma unroll
     for (int i = 0; i < N; i += 2) big = sm::fmax3(big, fabsf(__uint_as_float(r[i])), fabsf(__uint_as_float(r[i + 1])));
+    auto within = [&](float2 y) {
+        const float2 z = sm::mul2(y, y);
+        float2 x = sm::fma2(p.cap_poly[6], z, p.cap_poly[5]);
+#pragma unroll
+        for (int k = 4; k >= 0; --k) x = sm::fma2(x, z, p.cap_poly[k]);
+        return sm::mul2(x, y);
+    };
     if (__all_sync(0xffffffffu, big * fabsf(p.cap_inv) <= 1.f)) {
-        const float2 inv = make_float2(p.cap_inv, p.cap_inv);
 #pragma unroll
         for (int i = 0; i < N; i += 2) {
-            const float2 y = sm::mul2(make_float2(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), inv), z = sm::mul2(y, y);
-            float2 x = sm::fma2(p.cap_poly[6], z, p.cap_poly[5]);
-#pragma unroll
-            for (int k = 4; k >= 0; --k) x = sm::fma2(x, z, p.cap_poly[k]);
-            x = sm::mul2(x, y);
+            const float2 x = within(sm::mul2(make_float2(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), inv));
             r[i] = __float_as_uint(x.x);
             r[i + 1] = __float_as_uint(x.y);
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < N; ++i) r[i] = __float_as_uint(capped(p, __uint_as_float(r[i])));
+        for (int i = 0; i < N; i += 2) {
+            const float2 dot = make_float2(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), y = sm::mul2(dot, inv), x = within(y);
+            r[i] = __float_as_uint(fabsf(y.x) > 1.f ? capped(p, dot.x) : x.x);
+            r[i + 1] = __float_as_uint(fabsf(y.y) > 1.f ? capped(p, dot.y) : x.y);
+        }
     }
 }
 
