@@ -58,7 +58,8 @@ def attention(q, k_cache, v_cache, table, kv_lens, q_start, *, scale=1.0, taps=0
 
     The tolerance, with u = eps / 2 of the operands' type and w = 2^-23 (an fp32 operation, rounded in any direction):
       * a score is a sum of d products: off by (d + 8) w S at most, S = scale * max sum |q||k| + |bias|; probabilities
-        are off by that, relatively, and so is their sum;
+        are off by that, relatively, and so is their sum.  A cap's tanh does not enlarge what its argument is off by, and is off
+        by 8 w of its own value at most, which is no more than the score's;
       * n terms are summed up, and rescaled: (n + 64) w, for the numerator and for the denominator;
       * a probability rounded to the operands' 16 bits before it is multiplied: u of sum p |v| / sum p;
       * the result is rounded once: u of itself, and half of the smallest number of its type.
@@ -90,7 +91,6 @@ def attention(q, k_cache, v_cache, table, kv_lens, q_start, *, scale=1.0, taps=0
             mass = torch.einsum("hgd,nhd->hgn", x.abs(), k.abs()) * abs(scale)
             if softcap:
                 s = softcap * torch.tanh(s / softcap)
-                mass = mass + softcap
             if slopes is not None:
                 bias = slopes.double().view(heads, g, 1) * (i - j)
                 s, mass = s - bias, mass + bias.abs()

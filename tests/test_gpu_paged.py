@@ -155,6 +155,15 @@ def test_patterns_caps_and_bias(dtype, kw):
     check(x, scale=0.2, max_q_len=1, **kw)
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("softcap", [0.5, 50.0, 1e3, 1e5, 1e7, 1e30])
+def test_caps_far_from_the_scores(dtype, softcap):
+    """A capped score is as exact as its own size asks for, whatever the cap: single tokens, a few, and chunks."""
+    for d, heads in ((64, 8), (128, 4)):
+        check(batch(dtype, [(700, 1), (65, 1), (1, 1)], heads, 2, d, 16, seed=6), scale=d ** -0.5, softcap=softcap, max_q_len=1)
+        check(batch(dtype, [(300, 3), (257, 150)], heads, 2, d, 16, seed=7), scale=d ** -0.5, softcap=softcap)
+
+
 @pytest.mark.parametrize("dtype", [F16, BF16, F32])
 @pytest.mark.parametrize("lens, heads, kv_heads, d, page", [
     ([(128, 128)], 2, 2, 64, 16), ([(200, 129), (257, 31)], 4, 1, 128, 64), ([(640, 130), (1, 1), (90, 90), (700, 1)], 6, 2, 128, 32),

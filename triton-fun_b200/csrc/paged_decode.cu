@@ -367,10 +367,7 @@ paged_decode_kernel(const __grid_constant__ Maps maps, const __grid_constant__ P
                 const bool all_there = kChunk == 32 ? there == 0xffffffffu : (there & 0xffffu) == 0xffffu;
                 const bool inside = n0 >= inside_lo && n0 + kChunk <= inside_hi && all_there;
                 if (p.softcap > 0.f) {
-#pragma unroll
-                    for (int n = 0; n < kChunk / 8; ++n)
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) y[n][k] = capped(p, y[n][k]);
+                    cap_scores(p, reinterpret_cast<float (&)[kChunk / 2]>(y));
                 } else {
 #pragma unroll
                     for (int n = 0; n < kChunk / 8; ++n)
