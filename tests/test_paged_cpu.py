@@ -153,6 +153,16 @@ def test_attention_refusals(change, words, error):
     refused(r_paged.rpaged_attention_launcher, attention_args(), change, words, error)
 
 
+@pytest.mark.parametrize("change, words", [
+    (dict(scale=3e38), "scale must be at most 2e38"), (dict(scale=-3e38), "scale must be at most 2e38"), (dict(scale=2e38), "CUDA devices only"),
+    (dict(softcap=3e38), "too large for the scale"), (dict(softcap=1e38, scale=1e-3), "too large for the scale"),
+    (dict(softcap=1e38, scale=-1e-3), "too large for the scale"), (dict(softcap=1e38, scale=0.0), "CUDA devices only"),
+    (dict(softcap=1e30, scale=0.125), "CUDA devices only")])
+def test_scales_and_caps_whose_products_overflow_are_refused(change, words):
+    """2 log2 e softcap, log2 e scale and scale / softcap are what the kernels multiply with: infinite ones made NaN, tiny ones lost bits."""
+    refused(r_paged.rpaged_attention_launcher, attention_args(), change, words)
+
+
 def test_c_entry_points_refuse_bad_arguments():
     """Statuses of the C ABI for calls that launch nothing: null pointers, sizes that do not agree."""
     import ctypes

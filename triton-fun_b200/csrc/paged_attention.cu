@@ -459,7 +459,8 @@ static int32_t check_args(const splat_paged_args& a) {
     if (a.dtype != SPLAT_F32 && a.dtype != SPLAT_F16 && a.dtype != SPLAT_BF16) return SPLAT_ERR_UNSUPPORTED_DTYPE;
     if (a.tokens < 0 || a.requests < 0 || a.pages < 0 || a.page < 1 || a.heads < 1 || a.kv_heads < 1 || a.d < 1 || a.taps < 0 || a.stride < 1 ||
         a.table_width < 0 || a.table_stride < a.table_width || a.heads % a.kv_heads != 0 || !(a.softcap >= 0.f) ||
-        (a.softcap > 0.f && !std::isfinite(a.scale / a.softcap)))
+        (a.softcap > 0.f && !std::isfinite(a.scale / a.softcap)) || !(std::abs(a.scale) <= 2e38f) || a.softcap > 1e38f ||
+        (a.softcap > 0.f && a.scale != 0.f && std::abs(a.scale / a.softcap) < 1.2e-38f))
         return SPLAT_ERR_BAD_ARG;
     if (a.requests > SPLAT_PAGED_MAX_REQUESTS || a.d > 256 || a.pages > INT32_MAX || a.page > kMaxLen || a.table_width > kMaxLen ||
         a.table_width * a.page > kMaxLen || a.heads > 65535 || a.tokens >= kMaxLen / a.heads)

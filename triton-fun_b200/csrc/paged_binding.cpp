@@ -482,6 +482,10 @@ PyObject* paged_attention(PyObject* const* a, Py_ssize_t n) {
     x.softcap = number(a[11], "softcap");
     if (x.softcap < 0.f) refuse("softcap must not be negative");
     if (x.softcap > 0.f && !std::isfinite(x.scale / x.softcap)) refuse("softcap is too small for the scale");
+    // (scores are held in powers of two: log2 e and twice of it are in front of them)
+    if (std::abs(x.scale) > 2e38f) refuse("scale must be at most 2e38");
+    if (x.softcap > 1e38f || (x.softcap > 0.f && x.scale != 0.f && std::abs(x.scale / x.softcap) < 1.2e-38f))
+        refuse("softcap is too large for the scale: it caps nothing, leave it out");
     if (given(a[12])) {
         slopes = tensor(a[12], "slopes", 1);
         of_type(slopes, at::kFloat, "float32");
