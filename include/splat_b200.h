@@ -356,6 +356,7 @@ int32_t splat_debug_check_indices(int32_t* status_word);
  * entries), kv_lens = ctx + q, q_start (requests + 1, exclusive sums of q_lens), taken = {span[0] behind the step, span[1], pages
  * that were missing}, and for each of `tokens` rows its slot (page * page + row, or -1), position and request; rows behind
  * the last request get -1, 0 and -1.  A page that is missing (ring empty, table too narrow) leaves -1 in the table and the slots.
+ * Table entries, and taken, are those of all tokens, also of those that there is no row for.
  * Outputs may not overlap inputs; the inputs but block_table stay as they are. */
 int32_t splat_paged_tables(const int32_t* ctx_lens, const int32_t* q_lens, int32_t* block_table, int64_t table_stride,
                            const int32_t* ring, int64_t ring_size, const int64_t* span, int64_t page, int64_t requests,

@@ -65,6 +65,37 @@ def test_tables_without_requests_tokens_or_free_pages():
     assert got["slots"] == po.tables([0, 0], [5, 5], [[-7] * 4] * 2, list(range(9)), [0, 9], 2, 7)["slots"]
 
 
+@pytest.mark.parametrize("rows", [0, 1, 4, 7, 9, 10, 11])
+def test_tables_of_steps_with_more_tokens_than_rows(rows):
+    """Pages are taken for all of a step's tokens, so all of them stand in the table: none is lost."""
+    args = ([0, 3, 0], [5, 5, 40], 2, 9, list(range(50, 80)), [4, 30], rows, [[-7] * 9, [8, 9] + [-7] * 7, [-7] * 9])
+    assert run_tables(*args) == po.tables(args[0], args[1], args[7], args[4], args[5], args[2], rows)
+    rng = random.Random(rows)
+    ctx, new, page = [rng.randrange(60) for _ in range(700)], [rng.randrange(50) for _ in range(700)], 8
+    free = list(range(90000, 90000 + 3000))
+    got = run_tables(ctx, new, page, 12, free, [7, 3000], 1000 * rows)
+    assert got == po.tables(ctx, new, [[-7] * 12] * 700, free, [7, 3000], page, 1000 * rows)
+    # lengths that no table has room for
+    top = 2 ** 31 - 1
+    assert run_tables([0, 5], [top, top], 4, 3, [5, 6, 7, 8], [0, 4], rows)["table"] == [[5, 6, 7], [-7, -7, 8]]
+
+
+def test_a_step_with_more_tokens_than_the_module_has_rows_for():
+    """The requests that do not fit are not answered; their pages come back when they are released."""
+    m = r_paged.PagedAttention(12, 4, 2, 1, 64, 3, 8, 24, 0, BF16, scale=0.125)
+    x = [torch.randn(8, h, 64, device="cuda").to(BF16) for h in (2, 1, 1)]
+    m.begin_step(ints([0, 0, 0]), ints([5, 13, 1]))
+    m.output.fill_(7.0)
+    out = m(*x)
+    want, _, tol, _ = po.attention(x[0][:5], m.k_cache[0], m.v_cache[0], m.block_table[:1], m.kv_lens[:1], m.q_start[:2], scale=0.125)
+    assert bool(((out[:5].double() - want).abs() <= tol).all()) and bool((out[5:] == 7).all())
+    assert m.missing_pages() == 0 and m.free_span.tolist() == [7, 12]
+    for b, n in enumerate((5, 13, 1)):
+        m.release(b, n)
+    head, tail = m.free_span.tolist()
+    assert sorted(int(m.free_pages[i % 12]) for i in range(head, tail)) == list(range(12))
+
+
 def test_tables_of_the_longest_lengths():
     top = 2 ** 31 - 1
     got = run_tables([top, top], [1, 2], 1, 3, [5, 6], [0, 2], 3)

@@ -40,7 +40,8 @@ def rpaged_tables_launcher(ctx_lens: torch.Tensor, q_lens: torch.Tensor, block_t
     q_lens), for every row of tokens slots (int64: page * page_size + row), positions and requests (int32) -- rows behind the
     last request get -1, 0 and -1 -- and free_span_out (int64: what is left of free_span, and how many pages were
     missing).  A page that is missing, because the ring is empty or the table too narrow, leaves -1 in the table and
-    in the slots.  free_span_out is an array of its own, so that a call can be repeated."""
+    in the slots.  Pages are taken, and entered in the table, for all that q_lens says, also for tokens that slots has no row
+    for.  free_span_out is an array of its own, so that a call can be repeated."""
     _n.paged_tables(ctx_lens, q_lens, block_table, free_pages, free_span, page_size, kv_lens, q_start, slots, positions,
                     requests, free_span_out)
 
@@ -108,7 +109,9 @@ class PagedAttention(nn.Module):
         _n.status_word(dev)
 
     def begin_step(self, ctx_lens: torch.Tensor, q_lens: torch.Tensor, max_q_len=None) -> None:
-        """ctx_lens, q_lens: int32 (max_requests), tokens in the cache and new ones; 0 and 0 for a request that is not there."""
+        """ctx_lens, q_lens: int32 (max_requests), tokens in the cache and new ones; 0 and 0 for a request that is not there.
+        The new ones are max_tokens together at most: beyond them nothing is appended, and requests whose rows do not all fit are
+        not answered (``release`` them)."""
         rpaged_tables_launcher(ctx_lens, q_lens, self.block_table, self.free_pages, self.free_span, self.page_size,
                                self.kv_lens, self.q_start, self.slots, self.positions, self.requests, self.free_span_out)
         self.free_span.copy_(self.free_span_out[:2])

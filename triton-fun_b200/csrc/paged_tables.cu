@@ -8,7 +8,8 @@
 // What bounds it: nothing but latency (500 requests with 34 k new tokens: 0.6 MB; 4.3 us a launch behind another, as for 128 requests with one
 // token each).  So it is one launch without a second
 // phase: every block scans all lengths for itself, in shared memory, and then takes its share of the tokens; a token finds its request
-// by bisection in the scanned array.  A page's table entry is written by the token that stands in its first row, which is always a new one.
+// by bisection in the scanned array.  A page's table entry is written by the token that stands in its first row, which is always a new one; entries
+// of tokens that the caller has no row for (pages are taken for all that q_lens says) by a warp for each such request.
 #include "common.cuh"
 
 namespace splat {
@@ -56,6 +57,13 @@ __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* warp_sums, int
     __syncthreads();
     *whole = all;
     return before + x - v;
+}
+
+// Page that the k-th of a step's new table entries gets, or -1
+__device__ __forceinline__ int page_of(const TableArgs& a, int64_t first, int64_t avail, int64_t k) {
+    if (k >= avail) return -1;
+    const int64_t at = first + k;
+    return __ldg(a.ring + (at >= a.ring_size ? at - a.ring_size : at));
 }
 
 __global__ void __launch_bounds__(kThreads) paged_tables_kernel(const TableArgs a) {
@@ -126,17 +134,22 @@ __global__ void __launch_bounds__(kThreads) paged_tables_kernel(const TableArgs 
             if (i < held) {
                 page = *entry;
             } else {
-                const int64_t k = before[lo] + i - held;
-                if (k < avail) {
-                    const int64_t at = first + k;
-                    page = __ldg(a.ring + (at >= a.ring_size ? at - a.ring_size : at));
-                }
+                page = page_of(a, first, avail, before[lo] + i - held);
                 if (row == 0) *entry = page;
             }
         }
         a.slots[t] = page < 0 ? -1 : (int64_t)page * a.page + row;
         a.positions[t] = (int32_t)min(pos, (int64_t)INT32_MAX);
         a.token_request[t] = lo;
+    }
+    if (tokens <= a.tokens) return;
+    for (int b = (int)blockIdx.x * (kThreads / 32) + (int)(threadIdx.x >> 5); b < a.requests; b += (int)gridDim.x * (kThreads / 32)) {
+        const int64_t ctx = max(__ldg(a.ctx + b), 0), n = max(__ldg(a.fresh + b), 0), held = ceil_div(ctx, a.page);
+        if (start[b] + n <= a.tokens) continue;
+        const int64_t need = min(ceil_div(ctx + n, a.page), (int64_t)a.width);
+        for (int64_t i = held + (threadIdx.x & 31); i < need; i += 32)
+            if (start[b] + i * a.page - ctx >= a.tokens)           // (the place of the token in its first row)
+                a.table[(int64_t)b * a.table_stride + i] = page_of(a, first, avail, before[b] + i - held);
     }
 }
 
