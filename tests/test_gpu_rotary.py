@@ -174,3 +174,40 @@ def test_captured_forward_and_backward():
     graph.replay()
     close(a, po.rotary(q.detach(), pos, freq, cut), q.detach())
     close(g, po.rotary(dq, pos, freq, cut, inverse=True), dq)
+
+
+def test_tangents_in_forward_mode():
+    """The derivative along a tangent is the tangent, turned: of q, of k, of both, and with a gradient behind it."""
+    import torch.autograd.forward_ad as fwd
+    q, pos, freq, cut = inputs(torch.float32, 2, 4, 9, 32, 12, 2)
+    k = inputs(torch.float32, 2, 2, 9, 32, 12, 2, seed=1)[0]
+    dq, dk = (inputs(torch.float32, 2, h, 9, 32, 12, 2, seed=5 + h)[0].contiguous() for h in (4, 2))
+    want = [po.rotary(x, pos, freq, cut) for x in (q, k, dq, dk)]
+    with fwd.dual_level():
+        for with_q, with_k in ((True, True), (True, False), (False, True)):
+            a = fwd.make_dual(q, dq) if with_q else q
+            b = fwd.make_dual(k, dk) if with_k else k
+            for no_grad in (False, True):
+                with torch.set_grad_enabled(not no_grad):
+                    ya, yb = (fwd.unpack_dual(y) for y in r_rotary.rrotary(a, b, pos, freq, cut))
+                close(ya.primal, want[0], q)
+                close(yb.primal, want[1], k)
+                assert (ya.tangent is not None) == with_q and (yb.tangent is not None) == with_k
+                if with_q:
+                    close(ya.tangent, want[2], dq)
+                if with_k:
+                    close(yb.tangent, want[3], dk)
+        alone, none = r_rotary.rrotary(fwd.make_dual(q, dq), None, pos, freq, cut)
+        assert none is None
+        close(fwd.unpack_dual(alone).tangent, want[2], dq)
+        # a tangent of nothing but zeros, and one that has a gradient itself
+        zero = fwd.unpack_dual(r_rotary.rrotary(fwd.make_dual(q, torch._efficientzerotensor(q.shape, device="cuda")), None, pos, freq, cut)[0])
+        assert zero.tangent is None or not zero.tangent.any()
+        x, t = q.detach().clone().requires_grad_(True), dq.clone().requires_grad_(True)
+        y = fwd.unpack_dual(r_rotary.rrotary(fwd.make_dual(x, t), None, pos, freq, cut)[0])
+        gx, = torch.autograd.grad(y.primal, x, dq, retain_graph=True)
+        gt, = torch.autograd.grad(y.tangent, t, q)
+        close(gx, po.rotary(dq, pos, freq, cut, inverse=True), dq)
+        close(gt, po.rotary(q, pos, freq, cut, inverse=True), q)
+        with pytest.raises(ValueError, match="none for the frequencies"):
+            r_rotary.rrotary(q, None, pos, fwd.make_dual(freq, freq.clone()), cut)

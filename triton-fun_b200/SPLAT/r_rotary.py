@@ -24,5 +24,6 @@ def rrotary_launcher(q: torch.Tensor, k, positions: torch.Tensor, inv_freq: torc
 def rrotary(q: torch.Tensor, k, positions: torch.Tensor, inv_freq: torch.Tensor, sections=None, *,
             interleaved: bool = False):
     """``rrotary_launcher`` into new tensors, differentiable in q and k (also twice): (q', k'), k' None without k.  The
-    gradient of a rotation is the rotation by the opposite angle, one launch for both."""
+    gradient of a rotation is the rotation by the opposite angle, one launch for both; in forward mode the tangents are
+    turned like the operands, by a launch of their own."""
     return _n.rotary_grad(q, k, positions, inv_freq, sections, interleaved)

@@ -6,7 +6,11 @@
 #include <Python.h>
 
 #include <ATen/core/Tensor.h>
+#include <ATen/ops/_make_dual.h>
+#include <ATen/ops/_unpack_dual.h>
 #include <ATen/ops/empty.h>
+#include <ATen/ops/zeros.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -349,25 +353,51 @@ struct Rotary : torch::autograd::Function<Rotary> {
     }
 };
 
+// q and k (if defined) turned into y, differentiable in both; the tangents of dual tensors (forward mode) are turned as they are
+void turned(const at::Tensor& q, const at::Tensor& k, const at::Tensor& positions, const at::Tensor& inv_freq, const std::vector<int64_t>& sections,
+            bool interleaved, at::Tensor (&y)[2]) {
+    if (c10::AutogradState::get_tls_state().get_fw_grad_mode() && (q._fw_grad(0).defined() || (k.defined() && k._fw_grad(0).defined()))) {
+        at::Tensor x[2], t[2], dt[2];
+        for (int i = 0; i < 2; ++i) {
+            const at::Tensor& in = i == 0 ? q : k;
+            if (!in.defined()) continue;
+            std::tie(x[i], t[i]) = at::_unpack_dual(in, 0);
+            if (t[i].defined() && t[i]._is_zerotensor()) t[i] = at::zeros(t[i].sizes(), t[i].options());
+        }
+        turned(x[0], x[1], positions, inv_freq, sections, interleaved, y);
+        if (t[0].defined()) turned(t[0], t[1], positions, inv_freq, sections, interleaved, dt);
+        else turned(t[1], at::Tensor(), positions, inv_freq, sections, interleaved, dt);
+        if (!t[0].defined()) std::swap(dt[0], dt[1]);
+        for (int i = 0; i < 2; ++i)
+            if (dt[i].defined()) y[i] = at::_make_dual(y[i], dt[i], 0);
+        return;
+    }
+    if (at::GradMode::is_enabled() && (q.requires_grad() || (k.defined() && k.requires_grad()))) {
+        auto out = Rotary::apply(q, k.defined() ? std::optional<at::Tensor>(k) : std::nullopt, positions, inv_freq, sections, interleaved, false);
+        for (size_t i = 0; i < out.size(); ++i) y[i] = std::move(out[i]);
+        return;
+    }
+    Operand in[2] = {{&q, "q"}, {nullptr, nullptr}}, out[2] = {{nullptr, nullptr}, {nullptr, nullptr}};
+    if (k.defined()) in[1] = {&k, "k"};
+    rotate(in, out, y, {&positions, "positions"}, {&inv_freq, "inv_freq"}, sections, interleaved, 0);
+}
+
 // rotary_grad(q, k or None, positions, inv_freq, sections, interleaved) -> (q', k' or None), differentiable in q and k
 PyObject* rotary_grad(PyObject* const* a, Py_ssize_t n) {
     arguments(n, 6);
-    Operand in[2] = {tensor(a[0], "q", 4), {nullptr, nullptr}}, out[2] = {{nullptr, nullptr}, {nullptr, nullptr}};
-    if (given(a[1])) in[1] = tensor(a[1], "k", 4);
+    const Operand q = tensor(a[0], "q", 4);
+    const at::Tensor none;
+    Operand k{&none, "k"};
+    if (given(a[1])) k = tensor(a[1], "k", 4);
     const Operand positions = tensor(a[2], "positions"), inv_freq = tensor(a[3], "inv_freq", 1);
-    std::vector<int64_t> sections = sections_of(a[4]);
+    const std::vector<int64_t> sections = sections_of(a[4]);
     const int interleaved = flag(a[5]);
-    if (at::GradMode::is_enabled()) {
-        if (inv_freq->requires_grad()) refuse("inv_freq must not require a gradient: there is none for the frequencies");
-        if (in[0]->requires_grad() || (in[1].t != nullptr && in[1]->requires_grad())) {
-            const auto y = Rotary::apply(*in[0].t, in[1].t != nullptr ? std::optional<at::Tensor>(*in[1].t) : std::nullopt, *positions.t, *inv_freq.t,
-                                         std::move(sections), interleaved != 0, false);
-            return pair_of(wrapped(y[0]), wrapped(y.size() > 1 ? y[1] : at::Tensor()));
-        }
-    }
-    at::Tensor made[2];
-    rotate(in, out, made, positions, inv_freq, sections, interleaved, 0);
-    return pair_of(wrapped(made[0]), wrapped(made[1]));
+    if ((at::GradMode::is_enabled() && inv_freq->requires_grad()) ||
+        (c10::AutogradState::get_tls_state().get_fw_grad_mode() && inv_freq->_fw_grad(0).defined()))
+        refuse("inv_freq must not require a gradient: there is none for the frequencies");
+    at::Tensor y[2];
+    turned(*q.t, *k.t, *positions.t, *inv_freq.t, sections, interleaved != 0, y);
+    return pair_of(wrapped(y[0]), wrapped(y[1]));
 }
 
 struct Cache { int64_t pages, heads, page; };
