@@ -231,6 +231,35 @@ def test_queries_without_a_key(dtype):
     assert bool((check_rows[0][100] == 0).all())
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("new", [1, 3, 200])
+@pytest.mark.parametrize("page", [16, 7])
+def test_lengths_far_beyond_the_table(dtype, new, page):
+    """What a length claims behind the table's end is not there, and nothing walks over it: 2^30 keys would take seconds."""
+    full, T = -(-130 // page) * page, new + 1              # (rows that no token was written to would be seen, too)
+    x = batch(dtype, [(full, new), (40, 1)], 4, 2, 64, page, seed=9)
+    alone = {**x, "block_table": torch.cat((x["block_table"][:1].expand(new, -1), x["block_table"][1:])).contiguous(),
+             "kv_lens": ints([full] * new + [40]), "q_start": ints(list(range(T + 1)))}
+    want = po.attention(*(alone[k] for k in ("q", "k_cache", "v_cache", "block_table", "kv_lens", "q_start")), scale=0.2)
+    attend(x, scale=0.2)                                   # (the first call loads the kernels)
+    events = [torch.cuda.Event(enable_timing=True) for _ in range(2)]
+    for length in (10 ** 6, 2 ** 30 - 5, 2 ** 31 - 1):
+        x["kv_lens"][0] = length
+        for kw in (dict(), dict(max_q_len=new)):
+            torch.cuda.synchronize()
+            events[0].record()
+            out, lse = attend(x, scale=0.2, **kw)
+            events[1].record()
+            torch.cuda.synchronize()
+            assert events[0].elapsed_time(events[1]) < 20
+            assert bool(((out.double() - want[0]).abs() <= want[2]).all()) and bool(((lse.double() - want[1]).abs() <= want[3]).all())
+        out, lse = attend(x, scale=0.2, taps=60)           # a window behind everything that is there
+        assert bool((out[:new] == 0).all()) and bool((lse[:new] == float("-inf")).all()) and bool(lse[new:].isfinite().all())
+        for stride in (2, 64):
+            out, lse = attend(x, scale=0.2, stride=stride)
+            assert bool(lse.isfinite().all())
+
+
 def test_rows_of_no_request():
     x = batch(BF16, [(40, 7), (30, 1)], 4, 2, 64, 16, pad=9)
     check(x, scale=0.2)

@@ -120,7 +120,7 @@ __global__ void __launch_bounds__(kThreadsAny, kCols == 4 ? kPerSmAny : 2) paged
         const float slope = own_m >= 0 && p.slopes != nullptr ? p.slopes[head_of(own, own_m)] * kLog2e * (float)s : 0.f;
         const int m_first = token_of(0), m_last = min(p.group.div(w.tile * R + R - 1), t.count - 1);
         const int lo = max(m_first < 0 ? 0 : t.u0 + m_first - p.taps + 1, w.first_step() * kKeysAny);
-        const int hi = m_first < 0 ? 0 : min(t.u0 + m_last + 1, w.last_step() * kKeysAny);
+        const int hi = m_first < 0 ? 0 : min(min(t.u0 + m_last + 1, p.table_keys), w.last_step() * kKeysAny);
         float top = -INFINITY, sum = 0.f;                   // of the lane's row, over the stream's keys
         const T* kb = static_cast<const T*>(p.k) + w.head * p.k_head;
         const T* vb = static_cast<const T*>(p.v) + w.head * p.v_head;
@@ -577,6 +577,7 @@ extern "C" int32_t splat_paged_attention(const splat_paged_args* args, void* str
     p.group = FastDiv((uint32_t)(a.heads / a.kv_heads));
     p.stride = FastDiv((uint32_t)(a.stride < kMaxLen ? a.stride : kMaxLen));
     p.page_div = FastDiv((uint32_t)a.page);
+    p.table_keys = (int)((a.table_width * a.page + p.stride.d - 1) / p.stride.d);
     p.scale_log2 = a.scale * kLog2e;
     p.softcap = a.softcap * kLog2e;
     p.cap_inv = a.softcap > 0.f ? a.scale / a.softcap : 0.f;

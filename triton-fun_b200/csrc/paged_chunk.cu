@@ -174,7 +174,7 @@ paged_chunk_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Pr
             const RowPlace<kRows> rows(p, w, t);
             Piece x;
             x.lo = max(max(t.u0 + rows.first - p.taps + 1, 0), w.first_step() * kKeys);
-            x.hi = rows.first < t.count ? min(t.u0 + rows.last + 1, w.last_step() * kKeys) : 0;
+            x.hi = rows.first < t.count ? min(min(t.u0 + rows.last + 1, p.table_keys), w.last_step() * kKeys) : 0;
             x.first = x.lo / kKeys * kKeys;
             x.steps = x.hi > x.lo ? (x.hi - x.first + kKeys - 1) / kKeys : 0;
             x.u0 = t.u0; x.residue = t.residue; x.count = t.count; x.base = rows.base; x.head0 = rows.head0; x.row0 = (int)rows.row0;

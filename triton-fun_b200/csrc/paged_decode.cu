@@ -177,7 +177,7 @@ paged_decode_kernel(const __grid_constant__ Maps maps, const __grid_constant__ P
             const TileRows t = TileRows::of(p, w);
             const RowPlace<kRows> rows(p, w, t);
             const int lo = max(max(t.u0 + rows.first - p.taps + 1, 0), w.first_step() * S::kKeys);
-            const int hi = rows.first < t.count ? min(t.u0 + rows.last + 1, w.last_step() * S::kKeys) : 0;
+            const int hi = rows.first < t.count ? min(min(t.u0 + rows.last + 1, p.table_keys), w.last_step() * S::kKeys) : 0;
             const int limit = t.u0 + t.count;                  // keys of the class
             const int first = lo / kChunk * kChunk, chunks = hi > lo ? (hi - first + kChunk - 1) / kChunk : 0;
             const int head = w.head;

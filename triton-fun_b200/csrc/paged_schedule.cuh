@@ -21,7 +21,8 @@
 // worse than that (as a rule where there is less than one for each CTA), they are handed out whole.
 //
 // Steps are counted for a class of a request's longest kind, so that all of its classes and heads have the same tiles; where the count
-// is one too high a CTA has a step without keys.
+// is one too high a CTA has a step without keys.  They end where the block table does: what a length claims beyond it is not there, and is neither
+// counted nor walked over, whatever the length.
 #pragma once
 
 #include "common.cuh"
@@ -46,6 +47,7 @@ struct Problem {
     const float* slopes;
     int tokens, requests, pages, page, kv_heads, d;
     int table_rows;                    // tokens that the table has room for
+    int table_keys;                    // ... and keys of a class, one too many perhaps
     int taps;
     FastDiv group, stride, page_div;   // query heads per K/V head
     bool whole_tiles;                  // hand out tiles whole, whatever the lengths (and join nothing)
@@ -91,7 +93,7 @@ __device__ __forceinline__ Request request_of(const Problem& p, int b) {
 template <int R, int kKeys>
 __device__ __forceinline__ int2 steps_of(const Problem& p, const Request& r, int tile) {
     const int m_lo = p.group.div(tile * R), m_hi = min(p.group.div(tile * R + R - 1), r.longest - 1);
-    const int lo = max(0, r.u0 + m_lo - p.taps + 1), hi = r.u0 + m_hi + (p.stride.d > 1 ? 2 : 1);
+    const int lo = min(max(0, r.u0 + m_lo - p.taps + 1), p.table_keys), hi = min(r.u0 + m_hi + (p.stride.d > 1 ? 2 : 1), p.table_keys);
     const int x = lo / kKeys;
     return make_int2(x, max(x + 1, (hi + kKeys - 1) / kKeys));
 }
