@@ -250,3 +250,79 @@ def test_outputs_are_the_operands_themselves_or_elsewhere():
                           (dict(q_out=kw["k_cache"].view(6, 8, 16)[:5, :4]), "share memory"),
                           (dict(q=kw["k_cache"].view(6, 8, 16)[:5, :4]), "share memory")]:
         refused(r_paged.rpaged_append_launcher, kw, change, words)
+
+
+def test_outputs_that_start_elsewhere_in_an_operand_are_refused():
+    wide = torch.zeros(2, 4, 8, 16)
+    turn = dict(positions=i32(7), inv_freq=torch.zeros(8))
+    for kw, words in [(dict(q=wide[:, :, :-1], k=None, q_out=wide[:, :, 1:]), "q_out must be q itself"),
+                      (dict(q=wide[:, :, 1:], k=wide[:, :, :-1].clone(), k_out=wide[:, :, :-1]), "q must not share memory|k_out and q"),
+                      (dict(q=wide[:, 2:, 1:], k=wide[:, :2, 1:], q_out=wide[:, 2:, 1:], k_out=wide[:, :2, 1:]), "CUDA devices only"),
+                      (dict(q=wide[:, 2:, 1:], k=wide[:, :2, 1:], q_out=wide[:, :2, :-1], k_out=None), "q_out and k must not share")]:
+        refused(r_rotary.rrotary_launcher, {**turn, **kw}, {}, words)
+    kw = attention_args()
+    flat = torch.zeros(5 * 4 * 16 + 20 + 64)
+    out = flat[64:64 + 320].view(5, 4, 16)
+    f = dict(q=flat[:320].view(5, 4, 16), output=out)
+    refused(r_paged.rpaged_attention_launcher, kw, f, "output and q must not share")
+    for start in (0, 4, 300):
+        refused(r_paged.rpaged_attention_launcher, kw, dict(lse=kw["q"].view(-1)[start:start + 20].view(5, 4)), "lse and q must not share")
+        refused(r_paged.rpaged_attention_launcher, kw, dict(lse=kw["output"].view(-1)[start:start + 20].view(5, 4)), "output and lse must not share")
+    refused(r_paged.rpaged_attention_launcher, kw, dict(lse=flat[64:84].view(5, 4), slopes=flat[80:84]), "lse and slopes must not share")
+    refused(r_paged.rpaged_attention_launcher, kw, dict(block_table=kw["output"].view(torch.int32).view(-1)[3:11].view(2, 4)), "output and block_table")
+    kw = append_args()
+    refused(r_paged.rpaged_append_launcher, kw, dict(q_out=kw["k_cache"][1:].view(-1)[5 * 16:5 * 16 + 320].view(5, 4, 16)), "q_out and k_cache")
+    refused(r_paged.rpaged_append_launcher, kw, dict(v_cache=torch.zeros(5, 2, 8, 16)[1:4], k_cache=kw["k_cache"]), "CUDA devices only")
+    both = torch.zeros(4, 2, 8, 16)
+    refused(r_paged.rpaged_append_launcher, kw, dict(k_cache=both[:3], v_cache=both[1:]), "k_cache and v_cache must not share")
+    kw = tables_args()
+    line = i32(40)
+    refused(r_paged.rpaged_tables_launcher, kw, dict(kv_lens=line[:3], q_start=line[2:6]), "kv_lens and q_start must not share")
+    refused(r_paged.rpaged_tables_launcher, kw, dict(block_table=line[:24].view(3, 8)[:, :5], requests=line[10:17]), "block_table and requests")
+    refused(r_paged.rpaged_tables_launcher, kw, dict(block_table=line[:24].view(3, 8)[:, :5], kv_lens=line[5:8]), "CUDA devices only")
+
+
+def test_outputs_between_the_elements_of_operands_are_not_refused():
+    """Heads of a fused projection turned in place, K and V as halves of one array, rows of one page beside the others'."""
+    qkv = torch.zeros(5, 8, 16)
+    kw = {**append_args(), "q": qkv[:, :4], "k": qkv[:, 4:6], "v": qkv[:, 6:], "q_out": qkv[:, :4]}
+    both = torch.zeros(3, 2, 2, 8, 16)
+    rows = torch.zeros(3, 8, 4, 16)
+    for caches in ((both[:, 0], both[:, 1]), (rows[:, :, :2].transpose(1, 2), rows[:, :, 2:].transpose(1, 2))):
+        refused(r_paged.rpaged_append_launcher, kw, dict(k_cache=caches[0], v_cache=caches[1]), "CUDA devices only")
+    refused(r_paged.rpaged_append_launcher, kw, dict(q_out=qkv[:, 1:5]), "q_out must be q itself|q_out and k")
+    x = torch.zeros(2, 6, 7, 16)
+    refused(r_rotary.rrotary_launcher, dict(q=x[:, :4], k=x[:, 4:], q_out=x[:, :4], k_out=x[:, 4:], positions=i32(7), inv_freq=torch.zeros(8)), {},
+            "CUDA devices only")
+
+
+def test_shared_elements_against_sets_of_them():
+    """Random strided views of one small buffer, as operand and output: refused if and only if an element is both, or twice in the output."""
+    rng = random.Random(3)
+    buffer, where = torch.zeros(300), torch.arange(300)
+    seen = {"apart": 0, "itself": 0, "twice": 0, "shared": 0}
+    for _ in range(3000):
+        d = rng.choice([1, 2, 3])
+        size = [rng.randrange(1, 4) for _ in range(3)] + [d]
+
+        def view():
+            strides = [rng.choice([1, 2, 3, 4, 6, 9, 12, 18, 24, 36]) for _ in range(3)] + [1]
+            return size, strides, rng.randrange(0, 60)
+        a = view()
+        b = a if rng.random() < 0.1 else (a[0], a[1], rng.randrange(0, 60)) if rng.random() < 0.5 else view()
+        q, out = (buffer.as_strided(*v) for v in (a, b))
+        of_q, of_out = (where.as_strided(*v).reshape(-1).tolist() for v in (a, b))
+        real = [i for i in range(4) if size[i] > 1]
+        words = "CUDA devices only"
+        if len(set(of_out)) < len(of_out):
+            words, kind = "overlap itself", "twice"
+        elif not set(of_q) & set(of_out):
+            kind = "apart"
+        elif a[2] == b[2] and all(a[1][i] == b[1][i] for i in real):
+            kind = "itself"
+        else:
+            words, kind = "q_out must be q itself", "shared"
+        seen[kind] += 1
+        with pytest.raises(ValueError, match=words):
+            r_rotary.rrotary_launcher(q, None, i32(size[2]), torch.zeros(0), q_out=out)
+    assert min(seen.values()) > 50, seen

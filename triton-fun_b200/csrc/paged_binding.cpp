@@ -17,6 +17,7 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstdint>
 #include <optional>
@@ -98,10 +99,108 @@ void rows_contiguous(const Operand& x) {
 void contiguous(const Operand& x) {
     if (!x->is_contiguous()) refuse(std::string(x.name) + " must be contiguous");
 }
-// no element twice: what is written may not be an expanded tensor
+// ---- memory that operands share.  Outputs may interleave with other operands (heads of a fused projection, K and V as halves of one array), so
+// what counts is elements, not ranges.
+struct Steps { int64_t stride, lo, hi; };     // d strides, for any lo <= d <= hi
+// Whether a sum of d_k stride_k lies in [from, to]: steps in descending order of their strides (all above 0).  The steps of tensors, whose rows lie within
+// one another, leave two d_k to try at most; where that does not hold and `tries` run out, the answer is yes.
+bool reaches(const Steps* s, int n, int64_t from, int64_t to, int& tries) {
+    if (--tries < 0) return true;
+    int64_t lo = 0, hi = 0;                    // what the steps can add up to
+    for (int i = 0; i < n; ++i) {
+        lo += s[i].lo * s[i].stride;
+        hi += s[i].hi * s[i].stride;
+    }
+    if (lo > to || hi < from) return false;
+    if (n == 0) return true;
+    lo -= s[0].lo * s[0].stride;
+    hi -= s[0].hi * s[0].stride;
+    auto floor_div = [](int64_t a, int64_t b) { return a >= 0 ? a / b : -((b - 1 - a) / b); };
+    const int64_t first = std::max(s[0].lo, -floor_div(hi - from, s[0].stride)), last = std::min(s[0].hi, floor_div(to - lo, s[0].stride));
+    for (int64_t d = first; d <= last; ++d)
+        if (reaches(s + 1, n - 1, from - d * s[0].stride, to - d * s[0].stride, tries)) return true;
+    return false;
+}
+constexpr int kMaxSteps = 8, kTries = 4096;
+int add_steps(Steps* s, int n, const at::Tensor& t, int64_t sign) {
+    const auto size = t.sizes(), steps = t.strides();
+    const int64_t e = t.element_size();
+    for (size_t i = 0; i < size.size(); ++i) {
+        if (size[i] < 2 || steps[i] == 0) continue;
+        const int64_t stride = steps[i] * e, far = size[i] - 1;
+        int k = 0;
+        while (k < n && s[k].stride != stride) ++k;
+        if (k == n) s[n++] = {stride, 0, 0};
+        (sign > 0 ? s[k].hi : s[k].lo) += sign * far;
+    }
+    return n;
+}
+void descending(Steps* s, int n) {
+    std::sort(s, s + n, [](const Steps& a, const Steps& b) { return a.stride > b.stride; });
+}
+// no element twice in what is written
 void no_overlap(const Operand& x) {
+    const auto size = x->sizes(), steps = x->strides();
+    const int64_t e = x->element_size();
+    Steps s[kMaxSteps];
+    int n = 0;
+    for (size_t i = 0; i < size.size(); ++i) {
+        if (size[i] < 2) continue;
+        if (steps[i] == 0) refuse(std::string(x.name) + " must not be an expanded tensor");
+        int k = n++;                           // (descending)
+        for (; k > 0 && s[k - 1].stride < steps[i] * e; --k) s[k] = s[k - 1];
+        s[k] = {steps[i] * e, 0, size[i] - 1};
+    }
+    int64_t inner = e;                         // bytes of the steps behind
+    for (int k = n - 1; k >= 0; --k) {
+        if (s[k].stride < inner) {             // two elements whose first difference is in step k
+            Steps t[kMaxSteps] = {{s[k].stride, 1, s[k].hi}};
+            for (int i = k + 1; i < n; ++i) t[i - k] = {s[i].stride, -s[i].hi, s[i].hi};
+            int tries = kTries;
+            if (reaches(t, n - k, -(e - 1), e - 1, tries)) refuse(std::string(x.name) + " must not overlap itself");
+        }
+        inner += s[k].hi * s[k].stride;
+    }
+}
+struct Range { const char *begin, *end; };
+Range range_of(const Operand& x) {
+    if (x.t == nullptr || x->numel() == 0) return {nullptr, nullptr};
+    const char* begin = static_cast<const char*>(x->const_data_ptr());
+    if (begin == nullptr) return {nullptr, nullptr};
+    const auto size = x->sizes(), steps = x->strides();
+    int64_t far = 0;
+    for (size_t i = 0; i < size.size(); ++i) far += (size[i] - 1) * steps[i];
+    return {begin, begin + (far + 1) * static_cast<int64_t>(x->element_size())};
+}
+bool share_elements(const Operand& x, const Operand& y) {
+    Steps s[kMaxSteps];
+    const int n = add_steps(s, add_steps(s, 0, *x.t, 1), *y.t, -1);
+    descending(s, n);
+    const int64_t apart = static_cast<const char*>(x->const_data_ptr()) - static_cast<const char*>(y->const_data_ptr());
+    int tries = kTries;
+    return reaches(s, n, -(static_cast<int64_t>(x->element_size()) - 1) - apart, static_cast<int64_t>(y->element_size()) - 1 - apart, tries);
+}
+bool share(const Operand& x, const Range& rx, const Operand& y, const Range& ry) {
+    return rx.begin < ry.end && ry.begin < rx.end && share_elements(x, y);
+}
+bool is_itself(const Operand& x, const Operand& y) {
+    if (x->const_data_ptr() != y->const_data_ptr() || x->sizes() != y->sizes()) return false;
     for (int64_t i = 0; i < x->dim(); ++i)
-        if (x->size(i) > 1 && x->stride(i) == 0) refuse(std::string(x.name) + " must not be an expanded tensor");
+        if (x->size(i) > 1 && x->stride(i) != y->stride(i)) return false;
+    return true;
+}
+// Outputs (the first `outputs` of all; operands that are not there have no tensor) share memory with nobody, but where inputs[i] is given output i may be it.
+template <int N> void apart(const Operand (&all)[N], int outputs, std::initializer_list<const Operand*> inputs = {}) {
+    Range r[N];
+    for (int i = 0; i < N; ++i) r[i] = range_of(all[i]);
+    for (int i = 0; i < outputs; ++i) {
+        const Operand* own = i < static_cast<int>(inputs.size()) ? inputs.begin()[i] : nullptr;
+        for (int j = i + 1; j < N; ++j) {
+            if (!share(all[i], r[i], all[j], r[j])) continue;
+            if (own == nullptr || own->t != all[j].t) refuse(std::string(all[i].name) + " and " + all[j].name + " must not share memory");
+            if (!is_itself(all[i], all[j])) refuse(std::string(all[i].name) + " must be " + all[j].name + " itself or not share memory with it");
+        }
+    }
 }
 int device_of(std::initializer_list<Operand> all) {
     const Operand* first = nullptr;
@@ -113,16 +212,6 @@ int device_of(std::initializer_list<Operand> all) {
         else if (x->get_device() != (*first)->get_device()) refuse(std::string(x.name) + " and " + first->name + " are on different devices");
     }
     return (*first)->get_device();
-}
-void distinct(const Operand& x, const Operand& y) {
-    if (x->numel() > 0 && y->numel() > 0 && x->const_data_ptr() == y->const_data_ptr())
-        refuse(std::string(x.name) + " and " + y.name + " must not share memory");
-}
-// the same, unless x is y itself
-void itself_or_distinct(const Operand& x, const Operand& y) {
-    if (x->numel() == 0 || x->const_data_ptr() != y->const_data_ptr()) return;
-    for (int64_t i = 0; i < x->dim(); ++i)
-        if (x->size(i) > 1 && x->stride(i) != y->stride(i)) refuse(std::string(x.name) + " must be " + y.name + " itself or not share memory with it");
 }
 void check(int32_t rc, const char* what) {
     if (rc != 0)
@@ -159,15 +248,8 @@ PyObject* paged_tables(PyObject* const* a, Py_ssize_t n) {
     for (const Operand* x : {&ctx, &fresh, &ring, &span, &kv, &start, &slots, &positions, &requests, &taken}) contiguous(*x);
     rows_contiguous(table);
     if (B > 1 && table->stride(0) < table->size(1)) refuse("block_table: its rows must not overlap");
+    apart<11>({table, kv, start, slots, positions, requests, taken, ctx, fresh, ring, span}, 7);
     const int dev = device_of({ctx, fresh, table, ring, span, kv, start, slots, positions, requests, taken});
-    // outputs may be nobody else's memory (addresses first: asking the tensors for each pair takes longer than the launch)
-    const Operand* const all[] = {&table, &kv, &start, &slots, &positions, &requests, &taken, &ctx, &fresh, &ring, &span};
-    constexpr int kOutputs = 7, kAll = 11;
-    const void* at[kAll];
-    for (int i = 0; i < kAll; ++i) at[i] = (*all[i])->numel() > 0 ? (*all[i])->const_data_ptr() : nullptr;
-    for (int i = 0; i < kOutputs; ++i)
-        for (int j = i + 1; j < kAll; ++j)
-            if (at[i] != nullptr && at[i] == at[j]) distinct(*all[i], *all[j]);
     c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(dev));
     check(g_tables(data<int32_t>(ctx), data<int32_t>(fresh), data<int32_t>(table), B > 1 ? table->stride(0) : table->size(1),
                    data<int32_t>(ring), ring->size(0), data<int64_t>(span), page, B, table->size(1), T, data<int32_t>(kv),
@@ -258,10 +340,8 @@ void rotate(Operand (&in)[2], Operand (&out)[2], at::Tensor (&made)[2], const Op
         if (out[i]->sizes() != in[i]->sizes()) refuse(std::string(names[i]) + " must have the shape of its operand");
         rows_contiguous(out[i]);
         no_overlap(out[i]);
-        itself_or_distinct(out[i], in[i]);
-        if (count == 2) distinct(out[i], in[1 - i]);
     }
-    if (out[0].t != nullptr && out[1].t != nullptr) distinct(out[0], out[1]);
+    if (out[0].t != nullptr || out[1].t != nullptr) apart<6>({out[0], out[1], in[0], in[1], t.positions, t.inv_freq}, 2, {&in[0], &in[1]});
     const int dev = device_of({in[0], in[1], t.positions, t.inv_freq, out[0], out[1]});
     c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(dev));
     splat_rows rows[2] = {};
@@ -442,9 +522,6 @@ PyObject* paged_append(PyObject* const* a, Py_ssize_t n) {
         rows_contiguous(q);
         rows_contiguous(q_out);
         no_overlap(q_out);
-        itself_or_distinct(q_out, q);
-        for (const Operand* x : {&k, &v, &kc, &vc}) distinct(q_out, *x);
-        for (const Operand* x : {&kc, &vc}) distinct(*x, q);
     }
     Turn t;
     const bool turned = given(a[7]);
@@ -455,9 +532,8 @@ PyObject* paged_append(PyObject* const* a, Py_ssize_t n) {
         refuse("inv_freq without positions");
     }
     const int interleaved = flag(a[10]);
+    apart<9>({q_out, kc, vc, q, k, v, slots, t.positions, t.inv_freq}, 3, {&q});
     const int dev = device_of({k, v, kc, vc, slots, q, q_out, t.positions, t.inv_freq});
-    distinct(kc, vc);
-    for (const Operand* x : {&k, &v}) { distinct(kc, *x); distinct(vc, *x); }
     c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(dev));
     splat_rows rows[3] = {};
     int count = 0;
@@ -530,12 +606,8 @@ PyObject* paged_attention(PyObject* const* a, Py_ssize_t n) {
     }
     if (c.pages > INT32_MAX || table->size(1) > (1 << 30) / c.page || T >= (1 << 30) / H)
         refuse("pages, tokens of a request or tokens times heads beyond what the kernels count (2^31, 2^30)");
+    apart<9>({out, lse, q, kc, vc, table, kv, start, slopes}, 2);
     const int dev = device_of({q, kc, vc, table, kv, out, start, slopes, lse});
-    for (const Operand* y : {&q, &kc, &vc}) {
-        distinct(out, *y);
-        if (lse.t != nullptr) distinct(lse, *y);
-    }
-    if (lse.t != nullptr) distinct(lse, out);
     if (T == 0 || B == 0) Py_RETURN_NONE;
     c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(dev));
     if (x.dtype != SPLAT_F32) {
