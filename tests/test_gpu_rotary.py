@@ -83,6 +83,17 @@ def test_far_positions():
     close(r_rotary.rrotary_launcher(q, None, pos, freq)[0], po.rotary(q, pos[None, None], freq, cut), q)
 
 
+def test_cosines_and_sines_as_exact_as_fp32_has_them():
+    """The pairs (1, 0) come out as (cos, sin).  Functions off by one last place at most, 2^-24 below 1; one rounding more, half of one;
+    angles of up to 30000 radians in 64 bits, 2^-38."""
+    pos = torch.arange(30000, device="cuda", dtype=torch.int32)
+    freq = torch.tensor([10000.0 ** (-i / 32) for i in range(32)], device="cuda")
+    x = torch.cat((torch.ones(1, 1, 30000, 32, device="cuda"), torch.zeros(1, 1, 30000, 32, device="cuda")), -1)
+    got = r_rotary.rrotary_launcher(x, None, pos, freq)[0]
+    off = (got.double() - po.rotary(x, pos[None, None], freq, (32,))).abs()
+    assert float(off.max()) <= 1.5 * 2.0 ** -24 + 2.0 ** -38, float(off.max()) * 2 ** 24
+
+
 def test_empty_operands():
     freq = torch.ones(4, device="cuda")
     for shape in ((0, 2, 3, 8), (2, 0, 3, 8), (2, 2, 0, 8)):

@@ -17,7 +17,8 @@
 // every thread, walking over 22 heads: 69 / 23.
 //
 // The angle is formed in turns, in 64 bits: position times frequency of a far token has more than the 24 bits of fp32 in front
-// of its fraction.  cos and sin are of the fraction, in fp32, as are the products; they are rounded once, to the result's type.
+// of its fraction.  cos and sin are of the fraction's first 24 bits, in fp32; the rest of it, which is up to 2^-25 half turns (9e-8),
+// is added to first order: cos(a + b) = cos a - b sin a, sin(a + b) = sin a + b cos a.  Products are formed in fp32 and rounded once, to the result's type.
 #include "common.cuh"
 #include "fast_div.cuh"
 
@@ -145,8 +146,12 @@ __global__ void __launch_bounds__(kThreads, kPerSm) rotary_kernel(const __grid_c
         const int64_t where = axis * a.pos_axis + pb * a.pos_b + pl * a.pos_l;
         const int64_t pos = a.positions_64 ? static_cast<const int64_t*>(a.positions)[where] : static_cast<const int32_t*>(a.positions)[where];
         const double turns = (double)pos * (double)__ldg(a.inv_freq + pair) * 0.15915494309189533577;      // 1 / 2 pi
-        float2 cs;
-        sincospif((float)(2.0 * (turns - rint(turns))), &cs.y, &cs.x);
+        const double halves = 2.0 * (turns - rint(turns));
+        const float a0 = (float)halves, rest = (float)(halves - (double)a0) * 3.14159265f;
+        float2 cs0, cs;
+        sincospif(a0, &cs0.y, &cs0.x);
+        cs.x = fmaf(-rest, cs0.y, cs0.x);
+        cs.y = fmaf(rest, cs0.x, cs0.y);
         if (a.inverse) cs.y = -cs.y;
         angles[i] = cs;
     }
