@@ -235,6 +235,28 @@ def test_release_of_a_request_that_was_short_of_pages(row, length, freed):
         assert m.block_table.eq(-1).all()
 
 
+def module_on_the_cpu(table, page_size, pages, held):
+    """The tables of a PagedAttention that has handed out all but `held` of its pages, which lie in its ring from 8 on."""
+    m = r_paged.PagedAttention.__new__(r_paged.PagedAttention)
+    torch.nn.Module.__init__(m)
+    m.device, m.page_size = torch.device("cpu"), page_size
+    m.block_table = torch.tensor(table, dtype=torch.int32)
+    m.free_pages = torch.full((pages,), 77, dtype=torch.int32)
+    m.free_span = torch.tensor([8, 8 + len(held)])
+    for i, p in enumerate(held):
+        m.free_pages[(8 + i) % pages] = p
+    return m
+
+
+@pytest.mark.parametrize("length", [0, 3, 5, 8, 9, 28])
+def test_release_gives_all_pages_back_whatever_the_length(length):
+    """A request that dropped tokens has pages behind its length."""
+    m = module_on_the_cpu([[3, 1, -1, 4, -1, -1, -1], [0, 2, -1, -1, -1, -1, -1]], 4, 5, [])
+    m.release(0, length)
+    assert m.free_span.tolist() == [8, 11] and [int(m.free_pages[i % 5]) for i in range(8, 11)] == [3, 1, 4]
+    assert m.block_table.tolist() == [[-1] * 7, [0, 2, -1, -1, -1, -1, -1]]
+
+
 def test_outputs_are_the_operands_themselves_or_elsewhere():
     """In place means at the same strides: a row written before it is read as another one would be a wrong answer."""
     x = torch.zeros(2, 4, 4, 16)

@@ -136,12 +136,12 @@ class PagedAttention(nn.Module):
         return int(self.free_span_out[2])
 
     def release(self, request: int, length: int) -> None:
-        """Request `request` is done: the pages of its `length` tokens are free again, but for those that it never got."""
-        pages = -(-length // self.page_size)
+        """Request `request`, of `length` tokens, is done: all of its pages are free again, those of tokens that it did not keep
+        among them."""
         row = self.block_table[request]
-        if not 0 <= pages <= row.shape[0]:
+        if not 0 <= -(-length // self.page_size) <= row.shape[0]:
             raise ValueError("release: the request cannot have had so many tokens")
-        there = (row[:pages] >= 0).to(torch.int32)
+        there = (row >= 0).to(torch.int32)                 # (not those that it never got)
         order = torch.argsort(there, descending=True, stable=True)[:self.free_pages.shape[0]]
         at = (self.free_span[1] + torch.arange(order.shape[0], device=row.device)) % self.free_pages.shape[0]
         self.free_pages[at] = torch.where(there[order] > 0, row[order], self.free_pages[at])
