@@ -610,6 +610,54 @@ def test_serving_steps(dtype, kw):
     m.check_status()
 
 
+def test_drafted_tokens_that_are_refused():
+    """Steps of up to six drafted tokens of which some are kept: no page is lost, and what is kept is attended to."""
+    heads, kv_heads, d, page, B = 4, 2, 64, 4, 3
+    m = r_paged.PagedAttention(180, page, heads, kv_heads, d, B, 6 * B, 240, 0, BF16, scale=d ** -0.5)
+    rng, lens = random.Random(4), [0] * B
+    graph = None
+    lengths, drafts = ints([0] * B), ints([0] * B)
+    q, k, v = (torch.zeros(6 * B, h, d, device="cuda", dtype=BF16) for h in (heads, kv_heads, kv_heads))
+
+    def step():
+        m.rewind(lengths)
+        m.begin_step(lengths, drafts, 6)
+        m(q, k, v)
+    values = [[] for _ in range(B)]
+    for i in range(40):
+        new = [rng.randint(1, 6) for _ in range(B)]
+        for x in (q, k, v):
+            x.copy_(torch.randn(x.shape, device="cuda"))
+        lengths.copy_(ints(lens))
+        drafts.copy_(ints(new))
+        if i < 3:
+            step()
+        else:
+            if graph is None:
+                torch.cuda.synchronize()
+                graph = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(graph):
+                    step()
+            graph.replay()
+        assert m.missing_pages() == 0
+        head, tail = m.free_span.tolist()
+        entries = [e for row in m.block_table.tolist() for e in row if e >= 0]
+        free = [int(m.free_pages[j % 180]) for j in range(head, tail)]
+        assert sorted(entries + free) == list(range(180))
+        assert len(entries) == sum(-(-(a + b) // page) for a, b in zip(lens, new))
+        want, _, tol, _ = po.attention(q, m.k_cache[0], m.v_cache[0], m.block_table, m.kv_lens, m.q_start, scale=d ** -0.5)
+        n = sum(new)
+        assert bool(((m.output[:n].double() - want[:n]).abs() <= tol[:n]).all())
+        row = 0
+        for b in range(B):
+            kept = rng.randint(1, new[b])
+            values[b].append(v[row:row + kept].clone())
+            row += new[b]
+            lens[b] += kept
+            j = torch.arange(lens[b], device="cuda")
+            assert torch.equal(m.v_cache[0][m.block_table[b, j // page].long(), :, j % page], torch.cat(values[b]))
+
+
 def test_captured_serving_step():
     """A decoding step recorded once and replayed as the requests grow."""
     heads, kv_heads, d, page, B = 8, 2, 128, 16, 4

@@ -257,6 +257,19 @@ def test_release_gives_all_pages_back_whatever_the_length(length):
     assert m.block_table.tolist() == [[-1] * 7, [0, 2, -1, -1, -1, -1, -1]]
 
 
+@pytest.mark.parametrize("ctx, freed, left", [
+    ([16, 8], [], [[3, 1, -1, 4, -1], [0, 2, -1, -1, -1]]), ([13, 5], [], [[3, 1, -1, 4, -1], [0, 2, -1, -1, -1]]),
+    ([12, 5], [4], [[3, 1, -1, -1, -1], [0, 2, -1, -1, -1]]), ([4, 4], [1, 4, 2], [[3, -1, -1, -1, -1], [0, -1, -1, -1, -1]]),
+    ([0, -3], [3, 1, 4, 0, 2], [[-1] * 5] * 2), ([2 ** 31 - 1, 1], [2], [[3, 1, -1, 4, -1], [0, -1, -1, -1, -1]])])
+def test_rewind_gives_back_the_pages_behind_what_is_left(ctx, freed, left):
+    held = [5, 6]
+    m = module_on_the_cpu([[3, 1, -1, 4, -1], [0, 2, -1, -1, -1]], 4, 7, held)
+    for _ in range(2):                                     # (once more: nothing)
+        m.rewind(torch.tensor(ctx, dtype=torch.int32))
+        assert m.block_table.tolist() == left and m.free_span.tolist() == [8, 10 + len(freed)]
+        assert [int(m.free_pages[i % 7]) for i in range(8, 10 + len(freed))] == held + freed
+
+
 def test_outputs_are_the_operands_themselves_or_elsewhere():
     """In place means at the same strides: a row written before it is read as another one would be a wrong answer."""
     x = torch.zeros(2, 4, 4, 16)

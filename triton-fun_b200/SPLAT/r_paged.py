@@ -78,7 +78,8 @@ class PagedAttention(nn.Module):
     up to max_tokens new ones.
 
     A step: ``begin_step(ctx_lens, q_lens)`` once, then ``forward(q, k, v, layer)`` for every layer.  Rows of q, k and v are
-    the requests' new tokens behind one another; rows behind the last one are left alone.  ``forward`` returns the
+    the requests' new tokens behind one another; rows behind the last one are left alone.  ctx_lens are what the last step left, or 0
+    behind a ``release``, or less behind a ``rewind``.  ``forward`` returns the
     module-owned output buffer (the same tensor on every call).  Everything runs on the current stream without reading
     anything back and can be captured; two graphs that use one module share its buffers, so they may not run at the same time."""
 
@@ -141,12 +142,22 @@ class PagedAttention(nn.Module):
         row = self.block_table[request]
         if not 0 <= -(-length // self.page_size) <= row.shape[0]:
             raise ValueError("release: the request cannot have had so many tokens")
-        there = (row >= 0).to(torch.int32)                 # (not those that it never got)
-        order = torch.argsort(there, descending=True, stable=True)[:self.free_pages.shape[0]]
-        at = (self.free_span[1] + torch.arange(order.shape[0], device=row.device)) % self.free_pages.shape[0]
-        self.free_pages[at] = torch.where(there[order] > 0, row[order], self.free_pages[at])
-        self.free_span[1] += there.sum()
-        row.fill_(-1)
+        self._give_back(row, row >= 0)                     # (not those that it never got)
+
+    def rewind(self, ctx_lens: torch.Tensor) -> None:
+        """Requests go on behind ctx_lens tokens (int32, max_requests), fewer than they had where drafted tokens were refused: the
+        pages behind them are free again.  Before ``begin_step`` with these ctx_lens, which would take new pages in their place."""
+        held = (ctx_lens.clamp(min=0).long() + self.page_size - 1) // self.page_size
+        behind = torch.arange(self.block_table.shape[1], device=ctx_lens.device) >= held[:, None]
+        self._give_back(self.block_table.view(-1), (behind & (self.block_table >= 0)).view(-1))
+
+    def _give_back(self, entries: torch.Tensor, gone: torch.Tensor) -> None:
+        """Of the table's entries (a view) those that `gone` marks: pages to the end of the ring."""
+        order = torch.argsort(gone.to(torch.int32), descending=True, stable=True)[:self.free_pages.shape[0]]
+        at = (self.free_span[1] + torch.arange(order.shape[0], device=entries.device)) % self.free_pages.shape[0]
+        self.free_pages[at] = torch.where(gone[order], entries[order], self.free_pages[at])
+        self.free_span[1] += gone.sum()
+        entries.masked_fill_(gone, -1)
 
     def check_status(self) -> None:
         """Synchronises and raises if a kernel reported a wait that ran out."""
