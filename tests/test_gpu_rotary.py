@@ -139,6 +139,16 @@ def test_gradients(dtype, interleaved):
     assert bool(((g.double() - each.sum(0, keepdim=True)).abs() <= room).all())
 
 
+def test_gradients_with_a_sign_to_be_turned():
+    """The imaginary part of a conjugate is a view whose sign is not in memory."""
+    q, pos, freq, cut = inputs(torch.float32, 1, 2, 5, 16, 8, 1)
+    q.requires_grad_(True)
+    a, _ = r_rotary.rrotary(q, None, pos, freq, cut)
+    dq = torch.randn(q.shape, device="cuda", generator=torch.Generator(device="cuda").manual_seed(3))
+    g, = torch.autograd.grad(a, q, torch._neg_view(dq))
+    close(g, po.rotary(-dq, pos, freq, cut, inverse=True), dq)
+
+
 def test_gradient_against_differences():
     q, pos, freq, cut = inputs(torch.float32, 1, 2, 3, 16, 6, 2, far=50)
     q = q.contiguous().requires_grad_(True)
@@ -211,6 +221,8 @@ def test_tangents_in_forward_mode():
         alone, none = r_rotary.rrotary(fwd.make_dual(q, dq), None, pos, freq, cut)
         assert none is None
         close(fwd.unpack_dual(alone).tangent, want[2], dq)
+        turned = r_rotary.rrotary(fwd.make_dual(q.contiguous(), torch._neg_view(dq)), None, pos, freq, cut)[0]      # (a sign that is not in memory)
+        close(fwd.unpack_dual(turned).tangent, po.rotary(-dq, pos, freq, cut), dq)
         # a tangent of nothing but zeros, and one that has a gradient itself
         zero = fwd.unpack_dual(r_rotary.rrotary(fwd.make_dual(q, torch._efficientzerotensor(q.shape, device="cuda")), None, pos, freq, cut)[0])
         assert zero.tangent is None or not zero.tangent.any()

@@ -270,6 +270,15 @@ def test_rewind_gives_back_the_pages_behind_what_is_left(ctx, freed, left):
         assert [int(m.free_pages[i % 7]) for i in range(8, 10 + len(freed))] == held + freed
 
 
+def test_operands_that_are_not_what_their_memory_holds_are_refused():
+    """Views with a sign to be turned, and zeros without memory."""
+    for odd in (torch._neg_view(torch.ones(2, 4, 6, 16)), torch._efficientzerotensor((2, 4, 6, 16))):
+        for call in (r_rotary.rrotary, r_rotary.rrotary_launcher):
+            refused(call, rotary_args(), dict(q=odd), "values in memory", TypeError)
+        refused(r_paged.rpaged_attention_launcher, attention_args(), dict(q=odd[0, :, :5].transpose(0, 1)), "values in memory", TypeError)
+        refused(r_paged.rpaged_append_launcher, append_args(), dict(k=odd[0, :2, :5].transpose(0, 1)), "values in memory", TypeError)
+
+
 def test_outputs_are_the_operands_themselves_or_elsewhere():
     """In place means at the same strides: a row written before it is read as another one would be a wrong answer."""
     x = torch.zeros(2, 4, 4, 16)

@@ -52,6 +52,8 @@ Operand tensor(PyObject* o, const char* name, int64_t dims = -1) {
     if (o == nullptr || !THPVariable_Check(o)) throw Refused{PyExc_TypeError, std::string(name) + " must be a tensor"};
     const at::Tensor* t = &THPVariable_Unpack(o);
     if (t->layout() != at::kStrided) throw Refused{PyExc_TypeError, std::string(name) + " must be a strided tensor"};
+    if (t->is_neg() || t->is_conj() || t->_is_zerotensor())        // (not what its memory holds)
+        throw Refused{PyExc_TypeError, std::string(name) + " must hold its values in memory: see torch.resolve_neg and torch.clone"};
     if (dims >= 0 && t->dim() != dims) refuse(std::string(name) + " must be " + std::to_string(dims) + "-dimensional");
     return {t, name};
 }
@@ -393,6 +395,9 @@ PyObject* rotary(PyObject* const* a, Py_ssize_t n) {
     return pair_of(y[0], y[1]);
 }
 
+// A gradient or tangent that may be a view with its sign to be turned, or zeros without memory
+at::Tensor in_memory(const at::Tensor& t) { return t._is_zerotensor() ? at::zeros(t.sizes(), t.options()) : t.resolve_neg(); }
+
 // The same with gradients: that of a rotation is the rotation by the opposite angle.  In native code, since the Python form of such a
 // function takes as long as the kernels of ordinary calls do (fp32 B3 H12+4 L1369 d64, forward and backward: 97 us).
 struct Rotary : torch::autograd::Function<Rotary> {
@@ -415,7 +420,8 @@ struct Rotary : torch::autograd::Function<Rotary> {
         const auto saved = ctx->get_saved_variables();
         at::Tensor g[2], d[2];
         for (size_t i = 0; i < grads.size(); ++i) {
-            g[i] = grads[i];                               // (may come expanded, as that of a sum)
+            g[i] = grads[i];                               // (may come expanded, as that of a sum, and with its sign to be turned)
+            if (g[i].defined()) g[i] = in_memory(g[i]);
             if (g[i].defined() && g[i].size(-1) > 1 && g[i].stride(-1) != 1) g[i] = g[i].contiguous();
         }
         const int first = g[0].defined() ? 0 : 1;
@@ -442,7 +448,7 @@ void turned(const at::Tensor& q, const at::Tensor& k, const at::Tensor& position
             const at::Tensor& in = i == 0 ? q : k;
             if (!in.defined()) continue;
             std::tie(x[i], t[i]) = at::_unpack_dual(in, 0);
-            if (t[i].defined() && t[i]._is_zerotensor()) t[i] = at::zeros(t[i].sizes(), t[i].options());
+            if (t[i].defined()) t[i] = in_memory(t[i]);
         }
         turned(x[0], x[1], positions, inv_freq, sections, interleaved, y);
         if (t[0].defined()) turned(t[0], t[1], positions, inv_freq, sections, interleaved, dt);
