@@ -178,6 +178,19 @@ def test_c_entry_points_refuse_bad_arguments():
     assert lib.splat_paged_tables(none, none, none, 0, none, 1, none, 16, 20000, 0, 0, none, none, none, none, none, none, none) == -6
 
 
+def test_more_tokens_than_the_kernel_counts():
+    """Rows of 2^31 - 100 tokens and more: the last block's count passes 2^31 - 1.  (Nothing is launched, so any addresses do.)"""
+    import ctypes
+    import splat_native as n
+
+    class Rows(ctypes.Structure):
+        _fields_ = [("src", ctypes.c_void_p), ("dst", ctypes.c_void_p)] + [(f, ctypes.c_int64) for f in ("heads", "sb", "sh", "sl", "db", "dh", "dl")] + \
+                   [("turned", ctypes.c_int32), ("paged", ctypes.c_int32)]
+    rows = Rows(src=16, dst=16, heads=1, sl=2, dl=2)
+    for batch, length in ((1, 2 ** 31 - 1), (1, 2 ** 31 - 100), (2 ** 20, 2 ** 11), (3, 2 ** 30), (1, 2 ** 33)):
+        assert n._lib.splat_rotary(ctypes.byref(rows), 1, None, 0, 0, 0, 0, None, 0, None, 0, 0, 0, batch, length, 2, 0, None, 1, 0, None) == -6
+
+
 def test_module_refuses_the_cpu():
     with pytest.raises(ValueError, match="CUDA devices only"):
         r_paged.PagedAttention(4, 16, 4, 2, 64, 2, 8, 64, "cpu", torch.float16)

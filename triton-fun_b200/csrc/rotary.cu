@@ -190,7 +190,8 @@ int32_t launch(Args& a, cudaStream_t st) {
     a.turned_units = a.half / v;
     a.units = a.turned_units + (a.d - 2 * a.half) / v;
     const int64_t all = a.batch * a.length;
-    if (all > INT32_MAX || a.slots_end > INT32_MAX || a.length > INT32_MAX) return SPLAT_ERR_UNSUPPORTED_SHAPE;
+    // (the last block's tokens are counted past the end)
+    if (all > INT32_MAX - kThreads || a.slots_end > INT32_MAX || a.length > INT32_MAX) return SPLAT_ERR_UNSUPPORTED_SHAPE;
     // Heads of a thread: four in calls that fill the GPU (148 SMs with 1024 threads) twice over, else two (fp32 B3 H12+4 L1369 d64: 5.7 us, 8.3 with four)
     a.group_heads = all * a.units * a.heads >= (int64_t)8 * 148 * 1024 ? kHeads : 2;
     const int groups = (a.heads + a.group_heads - 1) / a.group_heads;
