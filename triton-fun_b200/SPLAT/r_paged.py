@@ -66,7 +66,8 @@ def rpaged_attention_launcher(q: torch.Tensor, k_cache: torch.Tensor, v_cache: t
     there are.  Scores: ``scale * q.k`` (default 1, as everywhere here), with ``softcap > 0`` capped to
     ``softcap * tanh(x / softcap)``, less ``slopes[head] * (i - j)`` if slopes (float32, heads) are given.  output (tokens,
     heads, d): softmax times V, zeros for a query without a key.  lse: float32 (tokens, heads), receives the natural
-    log-sum-exp of the scores, -inf without a key.  Rows that belong to no request are left as they are.  max_q_len: no
+    log-sum-exp of the scores, -inf without a key.  Scores and sums are held in 32 bits; with 16-bit operands probabilities are
+    rounded to their type before they are multiplied with V.  Rows that belong to no request are left as they are.  max_q_len: no
     request brings more tokens; it only helps to choose the kernel.  Returns output."""
     _n.paged_attention(q, k_cache, v_cache, block_table, kv_lens, output, q_start, max_q_len, scale, taps, stride, softcap,
                        slopes, lse)
@@ -112,7 +113,7 @@ class PagedAttention(nn.Module):
     def begin_step(self, ctx_lens: torch.Tensor, q_lens: torch.Tensor, max_q_len=None) -> None:
         """ctx_lens, q_lens: int32 (max_requests), tokens in the cache and new ones; 0 and 0 for a request that is not there.
         The new ones are max_tokens together at most: beyond them nothing is appended, and requests whose rows do not all fit are
-        not answered (``release`` them)."""
+        not answered (``release`` them).  max_q_len: no request brings more; without it kernels for long ones are launched, too."""
         rpaged_tables_launcher(ctx_lens, q_lens, self.block_table, self.free_pages, self.free_span, self.page_size,
                                self.kv_lens, self.q_start, self.slots, self.positions, self.requests, self.free_span_out)
         self.free_span.copy_(self.free_span_out[:2])

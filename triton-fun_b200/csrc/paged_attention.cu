@@ -23,8 +23,8 @@ __device__ __forceinline__ float score_of(const Problem& p, float dot) {
 // A tile is R rows: 8, or 4 or 2 where no request can have more.  kLanes lanes (16 for d <= 64, else the warp) hold a key: each has kCols of
 // its columns and of the rows' q and o.  The R dot products are added up over the lanes by halving: with 8 rows 4 + 2 + 1 exchanges leave
 // every lane with one row's sum over some lanes, one or two more complete it (8 to 9 shuffles for 8 sums; one by one they would be 32 to 40).
-// Issue slots bound it (56 % busy, HBM 64 %): 32 requests of 4096 tokens, 32 / 8 heads, d128 fp32 257 us, 4.2 TB/s; without the next keys on
-// their way 519.  A block's 4 warps are 4 or 8 streams that
+// 32 requests of 4096 tokens, 32 / 8 heads, d128 fp32 257 us, 4.2 TB/s; without the next keys on their way 519.  Neither issue slots (56 % busy) nor HBM
+// (64 %) are at an end: a stream's round is a chain of products, shuffles and exponentials, with 12 warps to an SM to cover it.  A block's 4 warps are 4 or 8 streams that
 // share a tile's keys and are joined at its end; K and V of a stream's next four keys are on their way while four are worked on.
 // -------------------------------------------------------------------------------------------------
 constexpr int kKeysAny = 32, kThreadsAny = 128, kPerSmAny = 3, kFixedAny = 3, kSplitAny = 1, kWholeAny = 3;
@@ -593,7 +593,9 @@ extern "C" int32_t splat_paged_attention(const splat_paged_args* args, void* str
         // second waits for the joining of the first
         if (chunk_rows(a) > kFewRows) {
             // One kernel for all of them where, as a rule, all bring as many, or where those of few rows are so few that a launch of their own
-            // costs more than tiles that are mostly empty (8 requests, 2 of them with chunks, 8 heads: the second kernel and its joining took 12 us)
+            // costs more than tiles that are mostly empty.  us, d128, 8 K/V heads, together / apart: 2 chunks of 512 over 4096 tokens among 8 requests 128 / 143,
+            // 16 151 / 163, 24 176 / 188, 48 250 / 254, 64 303 / 296; one of 64 over 512 among 16 21 / 38, 64 42 / 65.  (148 products of requests and heads
+            // are on the safe side.)
             const bool alike = a.tokens == a.requests * a.max_q_len || a.requests * a.kv_heads <= chunk_ctas(sms) / 2;
             p.rows_from = alike ? 0 : kFewRows + 1;
             const int32_t rc = attend_chunk(a, p, sms, a.workspace, st);

@@ -16,7 +16,7 @@
 //     a multiple of 8 rows; other pages and strides come by cp.async, 16 bytes each
 //     (32 requests of 4096 tokens, pages of 7 rows: 2.5 TB/s).  Pages are looked up for 32 boxes or keys at once.
 //   * A tile seldom has all 16 rows, and its end is spent on those that it has: with all of them joined, and written where a tile is divided,
-//     the same 85 (81: 5.5 TB/s, 0.84 of the measured copy rate), 96 windows of up to 1024 keys with 16 / 16 heads 80 (73), 96 requests of 128
+//     the same 85 (83: 5.3 TB/s, 0.82 of the measured copy rate), 96 windows of up to 1024 keys with 16 / 16 heads 80 (74: 0.72), 96 requests of 128
 //     tokens 35 (28).
 //   * Rows behind the request's last token, and of pages that are not there, are masked in S, and their rows of V are set to
 //     zero in the ring, whatever they held.

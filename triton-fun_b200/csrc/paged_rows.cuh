@@ -76,7 +76,7 @@ __device__ __forceinline__ float capped(const Problem& p, float dot) {
 
 // The same of scores in registers: up to the cap (as is the rule: caps of 30 to 50 and scores of some 10) c tanh y = c y P(y^2) on the FMA
 // units, two at a time, instead of two more special functions for each; beyond it as above.  P: the polynomial of degree 6 that
-// agrees with tanh(sqrt z) / sqrt z at the seven Chebyshev nodes of [0, 1]; off by 5e-8 of the value.
+// agrees with tanh(sqrt z) / sqrt z at the seven Chebyshev nodes of [0, 1]; off by 6e-8 of the value.
 // Which of the two a score takes is a matter of its own size alone.  Among a chunk's scores are keys that no row sees and columns that nothing was multiplied
 // into, with whatever memory held; they decide about the time (whether a warp looks for scores beyond the cap), never about a value.
 // us, bf16, 1024 tokens over 8192, 32 / 8 heads, d128: no cap 148; scores of about 1 and a cap of 50 221, of 1 350.
