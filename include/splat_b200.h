@@ -386,11 +386,12 @@ int32_t splat_rotary(const splat_rows* rows, int32_t n_rows, const void* positio
 
 /* Attention of new tokens over the paged cache.  Request b's queries are rows q_start[b] .. q_start[b + 1] - 1 of q, its last tokens:
  * query row t stands at position i = kv_lens[b] - q_start[b + 1] + t and attends to the keys j = i - k * stride >= 0, k < taps
- * (taps = 0: all of them).  Score: x = scale q.k, capped to softcap tanh(x / softcap) if softcap > 0 (scale / softcap
- * has to be finite, and not below the smallest normal number but where scale is 0; |scale| at most 2e38, softcap 1e38), less slopes[head] (i - j) if slopes is not null.  Query head h reads K/V head h / (heads / kv_heads).  o: softmax of the scores times V, 0 for a query without a
- * key; lse: (tokens, heads) float32 or null, the natural log-sum-exp of the scores, -inf for a query without a key.  Keys
- * end where the block table does, whatever kv_lens says; lengths beyond 2^30 count as 2^30.  Rows of q in
- * front of the first request and behind the last, and those of a request whose rows do not lie within [0, tokens), are left as they are. */
+ * (taps = 0: all of them).  Score: x = scale q.k, capped to softcap tanh(x / softcap) if softcap > 0, less slopes[head] (i - j) if slopes
+ * is not null.  |scale| is at most 2e38, softcap 1e38, and scale / softcap finite and, unless scale is 0, not below the smallest normal number.  Query
+ * head h reads K/V head h / (heads / kv_heads).  o: softmax of the scores times V, 0 for a query without a key; lse: (tokens, heads)
+ * float32 or null, the natural log-sum-exp of the scores, -inf for a query without a key.  Keys end where the block table does, whatever
+ * kv_lens says; lengths beyond 2^30 count as 2^30.  Rows of q in front of the first request and behind the last, and those of a request
+ * whose rows do not lie within [0, tokens), are left as they are. */
 typedef struct {
     const void *q, *k_cache, *v_cache;
     void* o;

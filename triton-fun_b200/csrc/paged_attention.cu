@@ -24,8 +24,9 @@ __device__ __forceinline__ float score_of(const Problem& p, float dot) {
 // its columns and of the rows' q and o.  The R dot products are added up over the lanes by halving: with 8 rows 4 + 2 + 1 exchanges leave
 // every lane with one row's sum over some lanes, one or two more complete it (8 to 9 shuffles for 8 sums; one by one they would be 32 to 40).
 // 32 requests of 4096 tokens, 32 / 8 heads, d128 fp32 257 us, 4.2 TB/s; without the next keys on their way 519.  Neither issue slots (56 % busy) nor HBM
-// (64 %) are at an end: a stream's round is a chain of products, shuffles and exponentials, with 12 warps to an SM to cover it.  A block's 4 warps are 4 or 8 streams that
-// share a tile's keys and are joined at its end; K and V of a stream's next four keys are on their way while four are worked on.
+// (64 %) are at an end: a stream's round is a chain of products, shuffles and exponentials, with 12 warps to an SM to cover it.
+// A block's 4 warps are 4 or 8 streams that share a tile's keys and are joined at its end; K and V of a stream's next four keys are on their
+// way while four are worked on.
 // -------------------------------------------------------------------------------------------------
 constexpr int kKeysAny = 32, kThreadsAny = 128, kPerSmAny = 3, kFixedAny = 3, kSplitAny = 1, kWholeAny = 3;
 

@@ -7,7 +7,8 @@
 //     O    += P(j) V(j)      tcgen05.mma 128xDx16, A = P from tensor memory, in two halves of 64 keys
 // At D = 128 P overwrites the scores and S(j + 1) follows PV(j); at D = 64 P has columns of its own and S(j + 1) is formed meanwhile.
 // The other CTA of the SM fills the gaps: a step takes a CTA 3.6 k cycles, 1.8 k with two side by side; tensor pipe 49 % busy.  1024 tokens over
-// 8192, 32 / 8 heads, d128 bf16: a call 148 us, 870 TFLOP/s; 2 x 2048 over 16384, at the power cap: 1210 to 1250 us, 855 to 825, by the card.  What is different here:
+// 8192, 32 / 8 heads, d128 bf16: a call 148 us, 870 TFLOP/s; 2 x 2048 over 16384, at the power cap: 1210 to 1250 us, 855 to 825, by the card.
+// What is different here:
 //   * A CTA walks over its share of all steps (paged_schedule.cuh), tile after tile, without a barrier of the block between them: the copying
 //     warp, which alone knows the schedule, runs ahead and hands the others a description of each piece of work through a ring of two.
 //   * K and V come in boxes of 8 to 128 rows, a lane of the copying warp to a box, which also looks up its page.

@@ -67,19 +67,26 @@ template <int R> struct RowPlace {
     __device__ __forceinline__ int64_t row_of(int m) const { return row0 + (int64_t)m * stride; }
 };
 
-// c tanh(x / c) in the log2 domain, with tanh y = 1 - 2 / (e^2y + 1): off by some 2^-22 of c, however small the score is.  So it is for scores beyond
-// the cap (|y| > 1), which are three quarters of c and more.
-__device__ __forceinline__ float capped(const Problem& p, float dot) {
-    const float e = sm::ex2(dot * p.cap_inv * (2.f * kLog2e));
-    return p.softcap - __fdividef(2.f * p.softcap, e + 1.f);
+// c tanh y of two scores in the log2 domain, with tanh y = 1 - 2 / (e^2y + 1), where |y| > 1; else x.  It is off by some 2^-22 of c however small the score
+// is, which is why it is for scores beyond the cap: three quarters of c and more.
+__device__ __forceinline__ float2 beyond_cap(const Problem& p, float2 y, float2 x) {
+    float2 e = sm::mul2(y, make_float2(2.f * kLog2e, 2.f * kLog2e));
+    e = sm::add2(make_float2(sm::ex2(e.x), sm::ex2(e.y)), make_float2(1.f, 1.f));
+    asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(e.x));
+    asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(e.y));
+    const float2 c = sm::fma2(e, make_float2(-2.f * p.softcap, -2.f * p.softcap), make_float2(p.softcap, p.softcap));
+    asm("{ .reg .pred q; setp.gt.f32 q, %1, 0f3F800000; selp.f32 %0, %2, %0, q; }" : "+f"(x.x) : "f"(fabsf(y.x)), "f"(c.x));
+    asm("{ .reg .pred q; setp.gt.f32 q, %1, 0f3F800000; selp.f32 %0, %2, %0, q; }" : "+f"(x.y) : "f"(fabsf(y.y)), "f"(c.y));
+    return x;
 }
 
 // The same of scores in registers: up to the cap (as is the rule: caps of 30 to 50 and scores of some 10) c tanh y = c y P(y^2) on the FMA
 // units, two at a time, instead of two more special functions for each; beyond it as above.  P: the polynomial of degree 6 that
 // agrees with tanh(sqrt z) / sqrt z at the seven Chebyshev nodes of [0, 1]; off by 6e-8 of the value.
 // Which of the two a score takes is a matter of its own size alone.  Among a chunk's scores are keys that no row sees and columns that nothing was multiplied
-// into, with whatever memory held; they decide about the time (whether a warp looks for scores beyond the cap), never about a value.
-// us, bf16, 1024 tokens over 8192, 32 / 8 heads, d128: no cap 148; scores of about 1 and a cap of 50 221, of 1 350.
+// into, with whatever memory held; they decide about the time (whether a warp looks for scores beyond the cap, 64 of a row at once), never about a value.
+// us, bf16, 1024 tokens over 8192, 32 / 8 heads, d128: no cap 148; cap 50 and scores of about 1 / 12 / 20 / 50: 225 / 323 / 338 / 327.  One vote for all 128: 225 / 389 /
+// 335 / 325 (code that seldom runs comes from beyond the instruction cache); a branch for each score instead of taking one of two: 221 / 465 / 358 / 351.
 constexpr float kTanhPoly[7] = {0.999999949f, -0.33332828f, 0.133250761f, -0.0534516464f, 0.0202797083f, -0.00619432483f, 0.0010380251f};
 __device__ __forceinline__ float score_bits(uint32_t x) { return __uint_as_float(x); }
 __device__ __forceinline__ float score_bits(float x) { return x; }
@@ -87,9 +94,6 @@ __device__ __forceinline__ void put_score(uint32_t& to, float x) { to = __float_
 __device__ __forceinline__ void put_score(float& to, float x) { to = x; }
 template <int N, typename E> __device__ __forceinline__ void cap_scores(const Problem& p, E (&r)[N]) {
     const float2 inv = make_float2(p.cap_inv, p.cap_inv);
-    float big = 0.f;
-#pragma unroll
-    for (int i = 0; i < N; i += 2) big = sm::fmax3(big, fabsf(score_bits(r[i])), fabsf(score_bits(r[i + 1])));
     auto within = [&](float2 y) {
         const float2 z = sm::mul2(y, y);
         float2 x = sm::fma2(p.cap_poly[6], z, p.cap_poly[5]);
@@ -97,19 +101,26 @@ template <int N, typename E> __device__ __forceinline__ void cap_scores(const Pr
         for (int k = 4; k >= 0; --k) x = sm::fma2(x, z, p.cap_poly[k]);
         return sm::mul2(x, y);
     };
-    if (__all_sync(0xffffffffu, big * fabsf(p.cap_inv) <= 1.f)) {
+    constexpr int kOnce = N < 64 ? N : 64;
 #pragma unroll
-        for (int i = 0; i < N; i += 2) {
-            const float2 x = within(sm::mul2(make_float2(score_bits(r[i]), score_bits(r[i + 1])), inv));
-            put_score(r[i], x.x);
-            put_score(r[i + 1], x.y);
-        }
-    } else {
+    for (int from = 0; from < N; from += kOnce) {
+        float big = 0.f;
 #pragma unroll
-        for (int i = 0; i < N; i += 2) {
-            const float2 dot = make_float2(score_bits(r[i]), score_bits(r[i + 1])), y = sm::mul2(dot, inv), x = within(y);
-            put_score(r[i], fabsf(y.x) > 1.f ? capped(p, dot.x) : x.x);
-            put_score(r[i + 1], fabsf(y.y) > 1.f ? capped(p, dot.y) : x.y);
+        for (int i = from; i < from + kOnce; i += 2) big = sm::fmax3(big, fabsf(score_bits(r[i])), fabsf(score_bits(r[i + 1])));
+        if (__all_sync(0xffffffffu, big * fabsf(p.cap_inv) <= 1.f)) {
+#pragma unroll
+            for (int i = from; i < from + kOnce; i += 2) {
+                const float2 x = within(sm::mul2(make_float2(score_bits(r[i]), score_bits(r[i + 1])), inv));
+                put_score(r[i], x.x);
+                put_score(r[i + 1], x.y);
+            }
+        } else {
+#pragma unroll
+            for (int i = from; i < from + kOnce; i += 2) {
+                const float2 y = sm::mul2(make_float2(score_bits(r[i]), score_bits(r[i + 1])), inv), x = beyond_cap(p, y, within(y));
+                put_score(r[i], x.x);
+                put_score(r[i + 1], x.y);
+            }
         }
     }
 }
